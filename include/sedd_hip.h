@@ -88,6 +88,25 @@ int sedd_predictor_step_philox(int graph, int step, const void* logscore, int dt
  * sedd_predictor_step; no counterpart in the reference (torch.rand_like, utils/catsample.py:12). */
 int sedd_philox_uniform(uint64_t seed, uint64_t offset, float* u, int64_t M, int Vu, sedd_stream_t stream);
 
+/* Truncated categorical sampling from given uniform numbers (NO COUNTERPART IN THE REFERENCE beyond the untruncated draw of
+ * utils/catsample.py:10-13).  Row r of `logits` ([M, V], row stride ld, unnormalised log-weights; -inf and NaN are never
+ * sampled) with the row's temperature T, top_k, top_p and min_p:
+ *   q_j  = exp((x_j - max x) / T);  rank by (x descending, index ascending)
+ *   kept = rank < top_k, and sum of q ranked before j < top_p * (sum of q over rank < top_k), and q_j >= min_p; rank 0 always
+ *   out  = argmax over kept of q_j / (1e-10 - log(min(u_j + 1e-10, 1)))  (u + 1e-10 rounded to fp32), lowest index of equals
+ * as 64-bit arithmetic decides it: rows near a border are decided in 64 bits, so the token depends on neither the kernel
+ * variant nor the batch.  T <= 0 (or NaN): the first maximum.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0: off.
+ * u fp32 [M, V] with row stride ldu, in [0, 1).  temperature / top_p / min_p fp32, top_k int32: one value per batch element
+ * (row r belongs to r / L), or NULL: the scalar beside it.  A row with nothing to sample gives -1.
+ * x (int64 [M], may be NULL): current tokens — only rows that hold mask_id are sampled, the others keep theirs, and a row with
+ * nothing to sample keeps mask_id.  move (fp32 per batch element, with x only, may be NULL): a masked row is sampled only
+ * where u[r][V] < move[r / L] (ldu >= V + 1 then): the ancestral update of an absorbing graph whose mask column is V.
+ * HBM bytes M (V (e + 4) + 8) over the sampled rows. */
+int sedd_sample_truncated(const void* logits, int dtype, int64_t ld, const float* u, int64_t ldu, const float* temperature,
+                          const int32_t* top_k, const float* top_p, const float* min_p, float temperature0, int top_k0,
+                          float top_p0, float min_p0, const int64_t* x, int64_t mask_id, const float* move, int64_t* out,
+                          int64_t M, int64_t L, int V, sedd_stream_t stream);
+
 /* Stand-alone Graph methods (for Graph-API parity; the predictor kernel above fuses them).  All outputs fp32
  * [M, V].  graph_lib.py:218-221/:139-145 (transp_rate), :79-93 (reverse_rate), :264-269/:162-165
  * (staggered_score), :226-234/:147-154 (transp_transition). score fp32 [M,V]; sig fp32 [B]. */
@@ -220,6 +239,33 @@ int sedd_gate_residual_ln_modulate_fwd(const float* residual, const void* a, int
                                        float inv_keep, uint64_t seed, float p_drop, const float* w, float* x_out,
                                        void* y, float* mean, float* rstd, int64_t M, int64_t L, int D,
                                        sedd_stream_t stream);
+
+/* The gated residual of a block whose branch output is normalised too, with a residual scale, and the next sub-layer's
+ * LayerNorm-modulate behind it, in one pass (transformer.py:185-186's pair with a norm AFTER the block as well; the norm of
+ * the branch output and the residual scale have no counterpart in the reference):
+ *   n = LN(a) * post_w;  x_out = res_scale * residual + gate_b * dropout(n);  y = LN(x_out) * w * (1 + scale_b) + shift_b
+ * residual / x_out fp32 [M, D]; a / y in a_dtype; gate / shift / scale rows of mod_dtype with row stride mod_stride;
+ * post_mean / post_rstd / mean / rstd fp32 [M] saved for backward.  w == NULL: no norm behind it (shift, scale, y, mean, rstd
+ * are not used).  Dropout by the (seed, p_drop) hash.  D % 4 == 0, D <= 2048. */
+int sedd_post_norm_residual_fwd(const float* residual, const void* a, int a_dtype, const float* post_w, const void* gate,
+                                const void* shift, const void* scale, int mod_dtype, int64_t mod_stride, float res_scale,
+                                float inv_keep, uint64_t seed, float p_drop, const float* w, float* x_out, void* y,
+                                float* post_mean, float* post_rstd, float* mean, float* rstd, int64_t M, int64_t L, int D,
+                                sedd_stream_t stream);
+/* its backward: dx1 fp32 [M, D] = the gradient of x_out that does not come through y (NULL: zero; with dh only), dh (a_dtype,
+ * or NULL: no norm behind) that of y.  d = dx1 + LayerNorm backward of dh;  dx = res_scale * d (dx may be dx1);  da (a_dtype) = the gradient of a.
+ * ws fp32 [6, nchunk, D] ([3, nchunk, D] without dh), nchunk = sedd_ln_bwd_chunks(M, L): partial column sums, folded by
+ * sedd_post_norm_residual_bwd_reduce into dgate [B, .] (row stride dgate_stride), dshift / dscale [B, .] (dmod_stride)
+ * (written), and dpost_w, dbias (the column sums of da before its rounding: the bias gradient of the Linear that made a), dw
+ * [D] (+=).  Any of them may be NULL.  Fixed order: bit-reproducible. */
+int sedd_post_norm_residual_bwd(const float* dx1, const void* dh, const float* x1, const float* w, const void* scale,
+                                const float* mean, const float* rstd, const void* a, int a_dtype, const float* post_w,
+                                const void* gate, int mod_dtype, int64_t mod_stride, const float* post_mean,
+                                const float* post_rstd, float res_scale, float inv_keep, uint64_t seed, float p_drop,
+                                float* dx, void* da, float* ws, int64_t M, int64_t L, int D, sedd_stream_t stream);
+int sedd_post_norm_residual_bwd_reduce(const float* ws, float* dgate, int64_t dgate_stride, float* dshift, float* dscale,
+                                       int64_t dmod_stride, float* dpost_w, float* dbias, float* dw, int64_t M, int64_t L,
+                                       int D, sedd_stream_t stream);
 
 /* Rotary (model/rotary.py:13-51): in-place NeoX rotation of the Q and K slots of qkv [B, L, 3, H, d]:
  * out = x*cos + rotate_half(x)*sin with rotate_half(x) = [-x2, x1]; conj != 0 applies the transposed rotation
@@ -440,6 +486,20 @@ int sedd_sumsq_clip(const float* g, int64_t n, float gscale, float max_norm, flo
  * squares that is already in out[0] — the sharded optimiser (reduce-scatter -> optimiser on the 1/N shard -> all-gather)
  * all-reduces the per-shard sums into out[0] first; clip_grad_norm_ of losses.py:65-66 over the WHOLE model. */
 int sedd_clip_from_sumsq(float* out, float gscale, float max_norm, sedd_stream_t stream);
+
+/* Gradients in many tensors (losses.py:65-66, torch.nn.utils.clip_grad_norm_ over a parameter list): out[0] = norm = sqrt of the
+ * sum of squares over all tensors (squares and sums in fp64, fixed order), out[1] = min(1, max_norm / (norm + 1e-6)); a NaN
+ * norm gives a NaN coefficient.  ptrs_host / numel_host / dtype_host are HOST arrays of ntensors entries, read before the
+ * call returns (the table travels as a launch argument: nothing is copied, a captured launch keeps its own); each tensor is
+ * dense, aligned to its type, fp32 or bf16.  ws: fp64 device scratch of SEDD_MULTI_WS_DOUBLES + ntensors doubles. */
+#define SEDD_MULTI_WS_DOUBLES 4096
+int sedd_multi_norm_clip(const void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host, int ntensors,
+                         float max_norm, double* ws, int64_t ws_doubles, float* out, sedd_stream_t stream);
+/* every tensor *= coef[0] in place (fp32 product rounded to the tensor's type); coef is one fp32 on the device, e.g. out + 1 of
+ * sedd_multi_norm_clip.  coef == 1 leaves the tensors unread.  round_coef != 0: bf16 tensors are multiplied by the coefficient
+ * as bf16 holds it (off by up to 2^-9), the value `grad.mul_(coef)` uses in a loop over the tensors. */
+int sedd_multi_scale(void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host, int ntensors,
+                     const float* coef, int round_coef, sedd_stream_t stream);
 
 #ifdef __cplusplus
 }

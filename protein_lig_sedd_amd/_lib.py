@@ -25,6 +25,7 @@ SIGNATURES = {
     "sedd_predictor_step": "iipippppllip",
     "sedd_predictor_step_philox": "iipippllpllip",
     "sedd_philox_uniform": "llplip",
+    "sedd_sample_truncated": "pilpl" + "pppp" + "fiff" + "plpp" + "llip",
     "sedd_transp_rate": "ipplip",
     "sedd_reverse_rate": "ippplip",
     "sedd_staggered_score": "ippplli" + "p",
@@ -46,6 +47,9 @@ SIGNATURES = {
     "sedd_gate_residual_bwd": "ppipilpflfppillip",
     "sedd_gate_residual_bwd_reduce": "pplp" + "llip",
     "sedd_gate_residual_ln_modulate_fwd": "ppipppil" + "flf" + "ppppp" + "llip",
+    "sedd_post_norm_residual_fwd": "ppipppp" + "il" + "fflf" + "ppp" + "pppp" + "llip",
+    "sedd_post_norm_residual_bwd": "ppppppp" + "pipp" + "ilpp" + "fflf" + "ppp" + "llip",
+    "sedd_post_norm_residual_bwd_reduce": "pplppl" + "ppp" + "llip",
     "sedd_rotary_qkv": "pippiiiiip",
     "sedd_gelu_fwd": "ppilp",
     "sedd_gelu_bwd": "pppilp",
@@ -80,6 +84,8 @@ SIGNATURES = {
     "sedd_clip_from_sumsq": "pffp",
     "sedd_ema_update": "ppflp",
     "sedd_batch_weighted_sum": "ppllppp",
+    "sedd_multi_norm_clip": "pppi" + "fplpp",
+    "sedd_multi_scale": "pppipip",
 }
 
 

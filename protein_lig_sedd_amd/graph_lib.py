@@ -185,5 +185,21 @@ class Absorbing(Graph):
             u = torch.rand(i.shape, dtype=torch.float32, device=i.device)
         return ops.sample_transition(self, i, sigma, u)
 
+    def ancestral_step(self, logscore, x, move=None, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One ancestral update: every masked position of x [B, L] is, with probability move (a number or [B]; None: all of
+        them, the final denoising), replaced by a token drawn from the log-scores [B, L, V] of the V - 1 tokens, truncated by
+        temperature, top-k, top-p and min-p (ops.sample_truncated); the other positions keep theirs.  u [B, L, V] uniform
+        noise whose last column decides who moves ([B, L, V - 1] without move); None draws torch.rand.  Without truncation
+        the update has the distribution of the Analytic predictor (sampling.py:88-99) under the model's own normalisation."""
+        V = self.dim
+        if logscore.shape[-1] != V:
+            raise ValueError(f"ancestral_step: log-scores over {logscore.shape[-1]} states, the graph has {V}")
+        Vu = V if move is not None else V - 1
+        if u is None:
+            u = torch.rand(*x.shape, Vu, dtype=torch.float32, device=x.device)
+        elif isinstance(u, ops.PhiloxNoise):
+            u = ops.philox_uniform(u, (*x.shape, Vu), x.device)
+        return ops.sample_truncated(logscore[..., :V - 1], u, temperature, top_k, top_p, min_p, x=x, mask_id=V - 1, move=move)
+
     def sample_limit(self, *batch_dims):
         return (self.dim - 1) * torch.ones(*batch_dims, dtype=torch.int64)

@@ -117,12 +117,36 @@ def get_optimizer(config, params):
     return FusedAdam(params, o.optimizer, float(o.lr), (o.beta1, o.beta2), o.eps, o.weight_decay)
 
 
+def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ (2-norm) of a parameter list, as losses.py:66 calls it, in a few launches over all of the
+    gradients (ops.clip_grad_norm_) -> the norm before clipping (0-dim fp32 tensor)."""
+    parameters = [parameters] if torch.is_tensor(parameters) else parameters
+    return ops.clip_grad_norm_([p.grad for p in parameters if p.grad is not None], max_norm, error_if_nonfinite)
+
+
 def optimization_manager(config):
-    """losses.py:49-71: warm-up -> clip -> optimiser step, here as one call into the bound trainer's fused step (the
-    GradScaler is accepted and ignored: bf16 / fp32 need no loss scaling)."""
+    """losses.py:49-71: warm-up -> clip -> optimiser step.  With the optimiser of `get_optimizer` this is one call into the
+    bound trainer's fused step (the GradScaler is accepted and ignored: bf16 / fp32 need no loss scaling); with an ordinary
+    torch optimiser — a subset of the parameters, another rule — it is the reference's sequence, the clipping over the
+    gradient tensors being `clip_grad_norm_`."""
 
     def optimize_fn(optimizer, scaler, params, step, lr=config.optim.lr, warmup=config.optim.warmup,
                     grad_clip=config.optim.grad_clip):
+        if isinstance(optimizer, torch.optim.Optimizer):
+            scaling = scaler is not None and scaler.is_enabled()
+            if scaling:
+                scaler.unscale_(optimizer)
+            if warmup > 0:
+                for g in optimizer.param_groups:
+                    g['lr'] = lr * min(step / warmup, 1.0)
+            if grad_clip >= 0:
+                clip_grad_norm_(params, grad_clip)
+            if scaling:
+                scaler.step(optimizer)
+                scaler.update()
+            else:
+                optimizer.step()
+            return
         tr = getattr(optimizer, "trainer", None)
         if tr is None:
             raise RuntimeError("optimize_fn needs a FusedAdam bound to a trainer (losses.get_step_fn binds it on its first call)")

@@ -221,7 +221,7 @@ class BlockLink:
     must be the very dx the next block returned — a second consumer of x2 (an activation hook feeding the loss) makes
     autograd sum into another tensor, which is detected and refused (SEDD_NO_BLOCK_CHAIN=1 then)."""
     __slots__ = ("norm1_w", "ada_w", "ada_b", "mlp2_bias", "mod", "h1", "mean1", "rstd1", "prev", "dy", "dmod_prev",
-                 "db2_fresh", "x2_key", "dx_key")
+                 "db2_fresh", "x2_key", "dx_key", "dpost_fresh")
 
     def __init__(self, prev_block, next_block):
         # next_block: a DDiTBlock, or the DDitFinalLayer behind the last block (its LayerNorm is `norm_final` and its
@@ -231,6 +231,7 @@ class BlockLink:
         self.mlp2_bias = prev_block.mlp[2].bias
         self.x2_key = self.dx_key = None
         self.mod = self.h1 = self.mean1 = self.rstd1 = self.prev = self.dy = self.dmod_prev = self.db2_fresh = None
+        self.dpost_fresh = None
 
     @staticmethod
     def key(t):
@@ -254,15 +255,39 @@ class BlockLink:
 BLOCK_CHAIN = not os.environ.get("SEDD_NO_BLOCK_CHAIN")  # A/B switch for the boundary fusion
 
 
+POST_PARAMS = ("post_norm1.weight", "post_norm2.weight")  # of a block whose branch outputs are normalised too
 BLOCK_PARAMS = ("norm1.weight", "attn_qkv.weight", "attn_out.weight", "norm2.weight", "mlp.0.weight", "mlp.0.bias",
                 "mlp.2.weight", "mlp.2.bias", "adaLN_modulation.weight", "adaLN_modulation.bias")
 
 
-def ddit_block_forward(x, c, P, n_heads, cos, sin, p_drop, cdt, save, cu_seqlens=None, link_in=None, link_out=None):
+def _post_norm_boundary_bwd(li, dh, x, w, scale, mean, rstd, dx, dw, dshift, dscale):
+    """A block boundary whose gated residual normalises its branch: the backward of the norm behind it (the next block's
+    norm1 or the final layer's) and of the previous block's last residual in one pass.  Fills the link (dy, dmod_prev, fresh
+    gradients) -> what the previous block's residual stream receives, its residual scale applied.  dx None: no gradient but
+    that of the norm."""
+    pv = li.prev
+    B, L, D = x.shape
+    W, pmean, prstd, alpha = pv["post"]
+    li.dmod_prev = torch.empty(B, 6 * D, dtype=torch.float32, device=x.device)
+    db2p, li.db2_fresh = _vec_sink(li.mlp2_bias, D)
+    dwp, li.dpost_fresh = _vec_sink(W, D)
+    dx, li.dy = ops.post_norm_residual_bwd(dx, pv["y"], W.detach(), pv["gate"], (pmean, prstd, mean, rstd),
+                                           li.dmod_prev[:, 5 * D:6 * D], dwp, pv["keep2"], pv["inv"], alpha,
+                                           norm=(dh, x, w, scale, dw, dshift, dscale), dbias=db2p)
+    li.dx_key = BlockLink.key(dx)
+    return dx
+
+
+def ddit_block_forward(x, c, P, n_heads, cos, sin, p_drop, cdt, save, cu_seqlens=None, link_in=None, link_out=None,
+                       res_scale=1.0):
     """DDiTBlock.forward (model/transformer.py:153-189).  x fp32 [B, L, D]; c fp32 [B, C]; P: dict of the block's
     parameters by reference name; cos/sin compact rotary tables.  Returns x_out fp32 and (if save) the saved state.
-    link_in / link_out: BlockLink with the previous / next block (None: stand-alone)."""
+    link_in / link_out: BlockLink with the previous / next block (None: stand-alone).
+    With post_norm{1,2}.weight among the parameters both branch outputs are normalised before their gate and the residual
+    stream is scaled by res_scale at each residual (ops.post_norm_residual_fwd)."""
     B, L, D = x.shape
+    post = "post_norm1.weight" in P
+    pst1 = pst2 = None
     M, H, d = B * L, n_heads, D // n_heads
     chained_in = link_in is not None and link_in.taken_by(x)
     c_c = None
@@ -287,7 +312,11 @@ def ddit_block_forward(x, c, P, n_heads, cos, sin, p_drop, cdt, save, cu_seqlens
     a = linear_fwd(o.view(M, D), P["attn_out.weight"]).view(B, L, D)
     inv = 1.0 / (1.0 - p_drop) if p_drop > 0 else 1.0
     keep1 = dropout_mask((B, L, D), p_drop, x.device) if p_drop > 0 else None
-    if ops.gate_residual_ln_modulate_supported(x, a, keep1):  # x1 and LN(x1) in one pass over the rows
+    if post:
+        x1, h2, pst1 = ops.post_norm_residual_fwd(x, a, P["post_norm1.weight"].detach(), mod[:, 2 * D:3 * D], keep1, inv,
+                                                  res_scale, norm=(w2, mod[:, 3 * D:4 * D], mod[:, 4 * D:5 * D]))
+        mean2, rstd2 = pst1[2:]
+    elif ops.gate_residual_ln_modulate_supported(x, a, keep1):  # x1 and LN(x1) in one pass over the rows
         x1, h2, mean2, rstd2 = ops.gate_residual_ln_modulate_fwd(x, a, mod[:, 2 * D:3 * D], keep1, inv, w2,
                                                                  mod[:, 3 * D:4 * D], mod[:, 4 * D:5 * D])
     else:
@@ -303,7 +332,7 @@ def ddit_block_forward(x, c, P, n_heads, cos, sin, p_drop, cdt, save, cu_seqlens
         g, u = linear_fwd(h2.view(M, D), P["mlp.0.weight"], P["mlp.0.bias"], gelu=True), None
     y = linear_fwd(g, P["mlp.2.weight"], P["mlp.2.bias"]).view(B, L, D)
     keep2 = dropout_mask((B, L, D), p_drop, x.device) if p_drop > 0 else None
-    chained_out = link_out is not None and ops.gate_residual_ln_modulate_supported(x1, y, keep2)
+    chained_out = link_out is not None and (post or ops.gate_residual_ln_modulate_supported(x1, y, keep2))
     if chained_out:  # x2 and the NEXT block's LayerNorm-modulate of it in one pass over the rows
         if c_c is None:
             c_c = c if cdt == torch.float32 else cast_once(c, cdt)
@@ -312,10 +341,20 @@ def ddit_block_forward(x, c, P, n_heads, cos, sin, p_drop, cdt, save, cu_seqlens
         else:  # the final layer's [B, 2D] modulation, at this block's row stride
             mod_n = torch.empty(B, 6 * D, dtype=cdt, device=x.device)[:, :link_out.ada_w.shape[0]]
             ops.gemm_nt(c_c, compute_weight(link_out.ada_w, cdt), bias=link_out.ada_b.detach(), out=mod_n)
-        x2, link_out.h1, link_out.mean1, link_out.rstd1 = ops.gate_residual_ln_modulate_fwd(
-            x1, y, mod[:, 5 * D:6 * D], keep2, inv, link_out.norm1_w.detach(), mod_n[:, :D], mod_n[:, D:2 * D])
+        if post:
+            x2, link_out.h1, pst2 = ops.post_norm_residual_fwd(
+                x1, y, P["post_norm2.weight"].detach(), mod[:, 5 * D:6 * D], keep2, inv, res_scale,
+                norm=(link_out.norm1_w.detach(), mod_n[:, :D], mod_n[:, D:2 * D]))
+            link_out.mean1, link_out.rstd1 = pst2[2:]
+        else:
+            x2, link_out.h1, link_out.mean1, link_out.rstd1 = ops.gate_residual_ln_modulate_fwd(
+                x1, y, mod[:, 5 * D:6 * D], keep2, inv, link_out.norm1_w.detach(), mod_n[:, :D], mod_n[:, D:2 * D])
         link_out.mod, link_out.x2_key = mod_n, BlockLink.key(x2)
-        link_out.prev = dict(y=y, gate=mod[:, 5 * D:6 * D], keep2=keep2, inv=inv) if save else None
+        link_out.prev = dict(y=y, gate=mod[:, 5 * D:6 * D], keep2=keep2, inv=inv,
+                             post=(P["post_norm2.weight"], *pst2[:2], res_scale) if post else None) if save else None
+    elif post:
+        x2, _, pst2 = ops.post_norm_residual_fwd(x1, y, P["post_norm2.weight"].detach(), mod[:, 5 * D:6 * D], keep2, inv,
+                                                 res_scale)
     else:
         x2 = ops.gate_residual_fwd(x1, y, mod[:, 5 * D:6 * D], keep2, inv)
     st = None
@@ -323,7 +362,7 @@ def ddit_block_forward(x, c, P, n_heads, cos, sin, p_drop, cdt, save, cu_seqlens
         st = dict(x=x, c=c, mod=mod, h1=h1, mean1=mean1, rstd1=rstd1, qkv=qkv, o=o, lse=lse, a=a, keep1=keep1,
                   x1=x1, h2=h2, mean2=mean2, rstd2=rstd2, u=u, u_grad=u_grad, g=g, y=y, keep2=keep2, inv=inv, cos=cos,
                   sin=sin, cu=cu_seqlens, link_in=link_in if chained_in else None,
-                  link_out=link_out if chained_out else None)
+                  link_out=link_out if chained_out else None, pst1=pst1, pst2=pst2, res_scale=res_scale)
     return x2, st
 
 
@@ -334,14 +373,24 @@ def ddit_block_backward(dx2, st, P, n_heads):
     M, H, d = B * L, n_heads, D // n_heads
     mod, cdt = st["mod"], st["h1"].dtype
     grads = {}
-    dx = torch.empty_like(dx2)  # = dx2 + both LN-branch gradients (dx2 itself is autograd's and stays untouched)
+    post = st.get("pst1") is not None
+    dx = None if post else torch.empty_like(dx2)  # = dx2 + both LN-branch gradients (dx2 is autograd's and stays untouched)
     # ---- MLP branch: x2 = x1 + gate_mlp * dropout(mlp(modulate(LN(x1))))
     lo = st.get("link_out")
     if lo is not None and lo.dy is not None:
         # the next block's norm1 backward already sent its finished dx (= dx2) through this gated residual's backward
         lo.check_grad(dx2)
         dy, dmod, grads["mlp.2.bias"] = lo.dy.view(M, D), lo.dmod_prev, lo.db2_fresh
-        lo.dy = lo.dmod_prev = lo.db2_fresh = lo.prev = None
+        if post:
+            grads["post_norm2.weight"] = lo.dpost_fresh
+        lo.dy = lo.dmod_prev = lo.db2_fresh = lo.dpost_fresh = lo.prev = None
+    elif post:
+        dmod = torch.empty(B, 6 * D, dtype=torch.float32, device=x.device)
+        db2, grads["mlp.2.bias"] = _vec_sink(P["mlp.2.bias"], D)
+        dwp, grads["post_norm2.weight"] = _vec_sink(P["post_norm2.weight"], D)
+        dx2, dy = ops.post_norm_residual_bwd(dx2, st["y"], P["post_norm2.weight"].detach(), mod[:, 5 * D:6 * D], st["pst2"],
+                                             dmod[:, 5 * D:6 * D], dwp, st["keep2"], st["inv"], st["res_scale"], dbias=db2)
+        dy = dy.view(M, D)
     else:
         dmod = torch.empty(B, 6 * D, dtype=torch.float32, device=x.device)
         db2, grads["mlp.2.bias"] = _vec_sink(P["mlp.2.bias"], D)  # column sums of dy ride along in the same pass
@@ -352,7 +401,14 @@ def ddit_block_backward(dx2, st, P, n_heads):
     dh2, grads["mlp.0.weight"], _ = linear_bwd(st["h2"].view(M, D), du, P["mlp.0.weight"], None)
     dw2, grads["norm2.weight"] = _vec_sink(P["norm2.weight"], D)
     # ---- attention branch: x1 = x + gate_msa * dropout(attn_out(attn(rotary(qkv(modulate(LN(x)))))))
-    if ops.gate_residual_ln_modulate_supported(st["x1"], st["a"], st["keep1"]) and dh2.dtype == st["a"].dtype:
+    if post:
+        dwp, grads["post_norm1.weight"] = _vec_sink(P["post_norm1.weight"], D)
+        dx, da = ops.post_norm_residual_bwd(dx2, st["a"], P["post_norm1.weight"].detach(), mod[:, 2 * D:3 * D], st["pst1"],
+                                            dmod[:, 2 * D:3 * D], dwp, st["keep1"], st["inv"], st["res_scale"],
+                                            norm=(dh2.view(B, L, D), st["x1"], P["norm2.weight"].detach(), mod[:, 4 * D:5 * D],
+                                                  dw2, dmod[:, 3 * D:4 * D], dmod[:, 4 * D:5 * D]))
+        da = da.view(M, D)
+    elif ops.gate_residual_ln_modulate_supported(st["x1"], st["a"], st["keep1"]) and dh2.dtype == st["a"].dtype:
         # norm2's backward and the gated residual's backward share one pass over the rows of dx
         da = ops.ln_modulate_bwd_gate(dh2.view(B, L, D), st["x1"], P["norm2.weight"].detach(), mod[:, 4 * D:5 * D],
                                       st["mean2"], st["rstd2"], dx, dx2, dw2, dmod[:, 3 * D:4 * D], dmod[:, 4 * D:5 * D],
@@ -375,7 +431,10 @@ def ddit_block_backward(dx2, st, P, n_heads):
     dh1, grads["attn_qkv.weight"], _ = linear_bwd(st["h1"].view(M, D), dqkv.view(M, 3 * D), P["attn_qkv.weight"])
     dw1, grads["norm1.weight"] = _vec_sink(P["norm1.weight"], D)
     li = st.get("link_in")
-    if li is not None and li.prev is not None and dh1.dtype == li.prev["y"].dtype:
+    if li is not None and li.prev is not None and li.prev["post"] is not None:
+        dx = _post_norm_boundary_bwd(li, dh1.view(B, L, D), x, P["norm1.weight"].detach(), mod[:, D:2 * D], st["mean1"],
+                                     st["rstd1"], dx, dw1, dmod[:, :D], dmod[:, D:2 * D])
+    elif li is not None and li.prev is not None and dh1.dtype == li.prev["y"].dtype:
         # block boundary: norm1's backward and the PREVIOUS block's last gated residual's backward (with its mlp[2] bias
         # gradient) share one pass over the rows of the finished dx
         pv = li.prev
@@ -431,10 +490,13 @@ def final_layer_backward(dlogits, st, P):
         dl = ops.cast(dl, cdt)
     dh, grads["linear.weight"], grads["linear.bias"] = linear_bwd(st["h"].view(M, D), dl, P["linear.weight"], P["linear.bias"])
     dmod = torch.empty(B, 2 * D, dtype=torch.float32, device=x.device)
-    dx = torch.empty_like(x)
     dw, grads["norm_final.weight"] = _vec_sink(P["norm_final.weight"], D)
     li = st.get("link_in")
-    if li is not None and li.prev is not None and dh.dtype == li.prev["y"].dtype:  # block boundary: see ddit_block_backward
+    dx = None if li is not None and li.prev is not None and li.prev["post"] is not None else torch.empty_like(x)
+    if dx is None:
+        dx = _post_norm_boundary_bwd(li, dh.view(B, L, D), x, P["norm_final.weight"].detach(), mod[:, D:2 * D], st["mean"],
+                                     st["rstd"], None, dw, dmod[:, :D], dmod[:, D:2 * D])
+    elif li is not None and li.prev is not None and dh.dtype == li.prev["y"].dtype:  # block boundary: see ddit_block_backward
         pv = li.prev
         li.dmod_prev = torch.empty(B, 6 * D, dtype=torch.float32, device=x.device)
         db2p, li.db2_fresh = _vec_sink(li.mlp2_bias, D)

@@ -140,10 +140,10 @@ class EmbeddingLayer(nn.Module):
 class _DDiTBlockFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, c, blk, cos, sin, save, cu, links, *params):
-        P = dict(zip(Lyr.BLOCK_PARAMS, params))
+        P = dict(zip(blk.param_names, params))
         p = blk.dropout if blk.training else 0.0
         out, st = Lyr.ddit_block_forward(x.contiguous(), c.contiguous(), P, blk.n_heads, cos, sin, p, blk.compute_dtype, save,
-                                         cu_seqlens=cu, link_in=links[0], link_out=links[1])
+                                         cu_seqlens=cu, link_in=links[0], link_out=links[1], res_scale=blk.residual_scale)
         ctx.st, ctx.P, ctx.n_heads, ctx.blk = st, P, blk.n_heads, blk
         return out
 
@@ -154,14 +154,27 @@ class _DDiTBlockFn(torch.autograd.Function):
         cb = getattr(ctx.blk, "_on_grads_ready", None)  # trainer hook: this block's gradient bucket is complete
         if cb is not None:
             cb()
-        return (dx, dc, None, None, None, None, None, None) + _ret(grads, Lyr.BLOCK_PARAMS)
+        return (dx, dc, None, None, None, None, None, None) + _ret(grads, ctx.blk.param_names)
 
 
 class DDiTBlock(nn.Module):
-    """transformer.py:118-189.  Same parameters / init; forward(x, rotary_cos_sin, c, seqlens=None)."""
+    """transformer.py:118-189.  Same parameters / init; forward(x, rotary_cos_sin, c, seqlens=None).
+    post_norm=True (not in the reference): the outputs of the attention and MLP branches are normalised too, by post_norm1 /
+    post_norm2 (LayerNorm with a weight), before their gate, and residual_scale multiplies the residual stream at each of
+    the two residuals: x <- residual_scale * x + gate * dropout(post_norm(branch(norm(x))))."""
 
-    def __init__(self, dim, n_heads, cond_dim, mlp_ratio=4, dropout=0.1, compute_dtype=torch.bfloat16):
+    def __init__(self, dim, n_heads, cond_dim, mlp_ratio=4, dropout=0.1, compute_dtype=torch.bfloat16, post_norm=False,
+                 residual_scale=1.0):
         super().__init__()
+        if residual_scale != 1.0 and not post_norm:
+            raise ValueError("DDiTBlock: residual_scale needs post_norm=True")
+        if post_norm and (dim % 4 or dim > 2048):
+            raise ValueError(f"DDiTBlock: post_norm needs a width that is a multiple of 4 and at most 2048, got {dim}")
+        self.residual_scale = float(residual_scale)
+        self.param_names = Lyr.BLOCK_PARAMS + (Lyr.POST_PARAMS if post_norm else ())
+        if post_norm:
+            self.post_norm1 = LayerNorm(dim)
+            self.post_norm2 = LayerNorm(dim)
         self.n_heads = n_heads
         self.norm1 = LayerNorm(dim)
         self.attn_qkv = nn.Linear(dim, 3 * dim, bias=False)
@@ -196,10 +209,10 @@ class DDiTBlock(nn.Module):
         packing); as in the reference the caller's `seqlens` therefore starts with 0 and sums to batch x seq_len, and the
         padded row length is the stated maximum segment length.  None: one segment per row."""
         cos, sin = self._tables(rotary_cos_sin)
-        P = _params(self, Lyr.BLOCK_PARAMS)
+        P = _params(self, self.param_names)
         cu = None if seqlens is None else seqlens.cumsum(-1).to(torch.int32).contiguous()
         return _DDiTBlockFn.apply(x, c, self, cos, sin, torch.is_grad_enabled(), cu, _links if cu is None else (None, None),
-                                  *[P[n] for n in Lyr.BLOCK_PARAMS])
+                                  *[P[n] for n in self.param_names])
 
 
 class _FinalLayerFn(torch.autograd.Function):
@@ -265,7 +278,8 @@ def _cfg(config, path, default=None):
 
 
 class _SEDD(nn.Module):
-    """transformer.py:332-392 (the plain upstream SEDD). forward(indices, sigma) -> log-score [B, L, V]."""
+    """transformer.py:332-392 (the plain upstream SEDD). forward(indices, sigma) -> log-score [B, L, V].
+    config.model.post_norm / config.model.residual_scale (optional): DDiTBlock's arguments of those names."""
 
     def __init__(self, config, compute_dtype=torch.bfloat16):
         super().__init__()
@@ -278,8 +292,11 @@ class _SEDD(nn.Module):
         self.vocab_embed = EmbeddingLayer(hidden, vocab_size)
         self.sigma_map = TimestepEmbedder(cond)
         self.rotary_emb = Rotary(hidden // heads)
+        res_scale = _cfg(config, "model.residual_scale")
         self.blocks = nn.ModuleList([
-            DDiTBlock(hidden, heads, cond, dropout=_cfg(config, "model.dropout"), compute_dtype=compute_dtype)
+            DDiTBlock(hidden, heads, cond, dropout=_cfg(config, "model.dropout"), compute_dtype=compute_dtype,
+                      post_norm=bool(_cfg(config, "model.post_norm", False)),
+                      residual_scale=1.0 if res_scale is None else float(res_scale))
             for _ in range(_cfg(config, "model.n_blocks"))
         ])
         self.output_layer = DDitFinalLayer(hidden, vocab_size, cond, compute_dtype=compute_dtype)

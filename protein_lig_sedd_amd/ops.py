@@ -1,6 +1,9 @@
 """Thin tensor-level wrappers over the C ABI (include/sedd_hip.h). Each takes/returns torch CUDA tensors, launches on
 torch's current stream and allocates outputs with torch's caching allocator. No arithmetic happens in Python."""
 import collections
+import contextlib
+import ctypes
+import math
 import os
 import threading
 
@@ -119,6 +122,22 @@ def _cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("protein_lig_sedd_amd ops need CUDA(HIP) tensors: there is no CPU fallback")
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on_device(t):
+    """`with` body: launches go to the stream that is current on t's device, whichever device is current."""
+    cur = _cur_device() if _cur_device is not None else torch.cuda.current_device()
+    return _SAME_DEVICE if t.device.index == cur else torch.cuda.device(t.device)
+
+
+def _one_device(name, *ts):
+    _cuda(*ts)
+    for t in ts:
+        if t is not None and t.device != ts[0].device:
+            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
 
 
 class SideStream:
@@ -348,6 +367,98 @@ def predictor_step_philox(graph, step, logscore, x, coef, noise):
         return predictor_step(graph, step, logscore, x, coef, u)
     check(rc, "sedd_predictor_step_philox")
     return out
+
+
+def _row_matrix(t, name):
+    """t [..., n] as rows of one stride: -> (tensor to keep, row stride in elements); copied if it is not laid out so."""
+    n = t.shape[-1]
+    rows = t.numel() // n if n else 0
+    ok, step = t.stride(-1) == 1 or n <= 1, None
+    for i in range(t.dim() - 2, -1, -1):
+        if t.shape[i] == 1:
+            continue
+        if step is None:
+            ld, step = t.stride(i), t.stride(i) * t.shape[i]
+        else:
+            ok, step = ok and t.stride(i) == step, step * t.shape[i]
+    if step is None:
+        ld = n
+    if not ok or (rows > 1 and ld < n):
+        t, ld = t.contiguous(), n
+    return t, ld
+
+
+def _per_request(v, B, dtype, device, name, lo, hi):
+    """a sampling parameter for all requests (a number) or one per request (a tensor [B], never read on the host)
+    -> (device tensor or None, number)"""
+    if torch.is_tensor(v):
+        if v.numel() not in (1, B):
+            raise ValueError(f"{name}: expected 1 or {B} values, got {v.numel()}")
+        if dtype == torch.int32 and v.dtype == torch.int64:
+            v = v.clamp(0, 2 ** 31 - 1)
+        v = v.detach().reshape(-1).to(device=device, dtype=dtype)
+        return (v if v.numel() == B else v.expand(B)).contiguous(), 0
+    if dtype == torch.int32:
+        if int(v) != v or v < lo:
+            raise ValueError(f"{name} must be a whole number >= {lo}, got {v}")
+        return None, min(int(v), 2 ** 31 - 1)
+    v = float(v)
+    if not lo <= v <= hi:
+        raise ValueError(f"{name} must lie in [{lo:g}, {hi:g}], got {v}")
+    return None, v
+
+
+def sample_truncated(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, x=None, mask_id=None, move=None):
+    """Categorical draw from logits [..., V] truncated by temperature, top-k, top-p and min-p (in this order), from given
+    uniform numbers u [..., V] -> int64 [...]; the definition stands at sedd_sample_truncated in include/sedd_hip.h.
+    temperature / top_k / top_p / min_p: a number, or a tensor with one value per entry of the leading dimension (one per
+    request).  temperature 0 takes the first maximum; top_k 0, top_p 1, min_p 0 switch the truncation off.  A row of -inf / NaN
+    only gives -1.
+    x [...] int64 with mask_id: rows whose token is not mask_id keep it.  move (with x; a number or one per leading entry):
+    a masked row is sampled only where the extra last column of u [..., V + 1] is below it."""
+    if logits.dim() < 1:
+        raise ValueError("sample_truncated: logits need a vocabulary dimension")
+    _one_device("sample_truncated", logits, u, x)
+    shape, V = logits.shape[:-1], logits.shape[-1]
+    B = shape[0] if len(shape) else 1
+    M = shape.numel()
+    if u.shape != (*shape, V if move is None else V + 1):
+        raise ValueError(f"sample_truncated: noise {tuple(u.shape)} for logits {tuple(logits.shape)}"
+                         + ("" if move is None else " and one more column for the move"))
+    if (x is None) != (mask_id is None):
+        raise ValueError("sample_truncated: x and mask_id come together")
+    if move is not None and x is None:
+        raise ValueError("sample_truncated: move needs x and mask_id")
+    if x is not None and x.shape != shape:
+        raise ValueError(f"sample_truncated: x {tuple(x.shape)} for logits {tuple(logits.shape)}")
+    dev = logits.device
+    T, T0 = _per_request(temperature, B, torch.float32, dev, "temperature", 0.0, 3.4e38)
+    k, k0 = _per_request(top_k, B, torch.int32, dev, "top_k", 0, 0)
+    P, P0 = _per_request(top_p, B, torch.float32, dev, "top_p", 0.0, 1.0)
+    m, m0 = _per_request(min_p, B, torch.float32, dev, "min_p", 0.0, 1.0)
+    dt = _dt(logits)
+    with _on_device(logits):
+        if move is not None:
+            move = _per_request(move, B, torch.float32, dev, "move", 0.0, 1.0)
+            move = move[0] if move[0] is not None else torch.full((B,), move[1], dtype=torch.float32, device=dev)
+        logits, ld = _row_matrix(logits, "logits")
+        u, ldu = _row_matrix(u if u.dtype == torch.float32 else u.float(), "u")
+        x = _c(x, torch.int64)
+        out = torch.empty(shape, dtype=torch.int64, device=dev)
+        with _Timed("sample_truncated", float(M) * (V * (logits.element_size() + 4) + 8)):
+            check(lib().sedd_sample_truncated(_p(logits), dt, ld, _p(u), ldu, _p(T), _p(k), _p(P), _p(m), T0, k0, P0, m0,
+                                              _p(x), -1 if mask_id is None else int(mask_id), _p(move), _p(out), M,
+                                              max(M // max(B, 1), 1), V, _stream()), "sedd_sample_truncated")
+    return out
+
+
+def philox_uniform(noise, shape, device):
+    """the uniform numbers a PhiloxNoise stands for, as a tensor [..., columns]"""
+    u = torch.empty(shape, dtype=torch.float32, device=device)
+    seed = noise.seed - (1 << 64) if noise.seed >= (1 << 63) else noise.seed
+    check(lib().sedd_philox_uniform(seed, noise.offset, _p(u), u.numel() // max(shape[-1], 1), shape[-1], _stream()),
+          "sedd_philox_uniform")
+    return u
 
 
 def transp_rate(graph, x):
@@ -648,6 +759,105 @@ def gate_residual_bwd(dout, a, gate, dgate, keep=None, inv_keep=1.0, dbias=None)
     elif dbias is not None:
         raise ValueError("gate_residual_bwd: dbias rides on the gate gradient's fold")
     return da
+
+
+def _post_norm_args(name, residual, a, post_w, gate, keep, norm):
+    """checks shared by post_norm_residual_fwd / _bwd -> (B, L, D, gate, modulation dtype, row stride, seed, p_drop)"""
+    if residual.dim() != 3 or residual.dtype != torch.float32 or not residual.is_contiguous():
+        raise ValueError(f"{name}: the residual stream must be contiguous fp32 [B, L, D]")
+    B, L, D = residual.shape
+    if a.shape != residual.shape or not a.is_contiguous():
+        raise ValueError(f"{name}: the branch output must be contiguous {tuple(residual.shape)}, got {tuple(a.shape)}")
+    for w in (post_w,) + ((norm[0],) if norm is not None else ()):
+        if w.shape != (D,) or w.dtype != torch.float32 or not w.is_contiguous():
+            raise ValueError(f"{name}: norm weights must be contiguous fp32 [{D}]")
+    g, mdt, ms = _mod_args(gate)
+    for t in (gate,) + (tuple(norm[1:]) if norm is not None else ()):
+        if t.shape != (B, D) or (B > 1 and t.stride(0) != ms) or _mod_args(t)[1] != mdt or t.data_ptr() % (4 * t.element_size()):
+            raise ValueError(f"{name}: gate / shift / scale must be [{B}, {D}] slices of one modulation dtype and row stride")
+    if keep is not None and not isinstance(keep, DropSeed):
+        raise ValueError(f"{name}: dropout by DropSeed only")
+    _, seed, pd = _keep_args(keep)
+    return B, L, D, g, mdt, ms, seed, pd
+
+
+def post_norm_residual_fwd(residual, a, post_w, gate, keep=None, inv_keep=1.0, res_scale=1.0, norm=None):
+    """x1 = res_scale * residual + gate * dropout(LN(a) * post_w) and, with norm = (w, shift, scale),
+    h = LN(x1) * w * (1 + scale) + shift, in one pass over the rows.  residual fp32 [B, L, D]; a [B, L, D]; gate / shift / scale
+    [B, D] slices of modulation tensors of one row stride; keep: DropSeed or None.
+    -> (x1 fp32, h in a's dtype or None, (post_mean, post_rstd, mean, rstd) [M] for the backward; the last two None without norm)."""
+    ts = (residual, a, post_w, gate) + (tuple(norm) if norm is not None else ())
+    _one_device("post_norm_residual_fwd", *ts)
+    w, shift, scale = norm if norm is not None else (None, None, None)
+    B, L, D, g, mdt, ms, seed, pd = _post_norm_args("post_norm_residual_fwd", residual, a, post_w, gate, keep,
+                                                    None if norm is None else norm)
+    M = B * L
+    with _on_device(residual):
+        x1 = torch.empty_like(residual)
+        h = torch.empty_like(a) if norm is not None else None
+        st = torch.empty(4 if norm is not None else 2, M, dtype=torch.float32, device=residual.device)
+        stats = (st[0], st[1], st[2], st[3]) if norm is not None else (st[0], st[1], None, None)
+        with _Timed("post_norm_residual_fwd", float(M) * D * (8 + a.element_size() * (1 if norm is None else 2))):
+            check(lib().sedd_post_norm_residual_fwd(_p(residual), _p(a), _dt(a), _p(post_w), _p(g), _p(shift), _p(scale), mdt,
+                                                    ms, float(res_scale), float(inv_keep), seed, pd, _p(w), _p(x1), _p(h),
+                                                    *[_p(t) for t in stats], M, max(L, 1), D, _stream()),
+                  "sedd_post_norm_residual_fwd")
+    return x1, h, stats
+
+
+def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=None, inv_keep=1.0, res_scale=1.0, norm=None,
+                           dbias=None):
+    """Backward of post_norm_residual_fwd -> (dx fp32, da in a's dtype).  dx1: the gradient of x1 from the residual stream
+    (None, with norm only: zero); stats: the forward's.  norm = (dh, x1, w, scale, dw, dshift, dscale): the next norm's incoming gradient dh, its saved x1,
+    weight and scale, and where its gradients go.  dgate / dshift / dscale fp32 [B, D] (strided) are written; dpost_w, dw and
+    dbias (column sums of da before its rounding: the bias gradient of the Linear that made a) fp32 [D] are accumulated.
+    dgate, dpost_w, dbias, dw, dshift, dscale may be None."""
+    dh, x1, w, scale, dw, dshift, dscale = norm if norm is not None else (None,) * 7
+    if dx1 is None and norm is None:
+        raise ValueError("post_norm_residual_bwd: dx1 None needs a norm")
+    like = x1 if dx1 is None else dx1
+    _one_device("post_norm_residual_bwd", like, dx1, a, post_w, gate, *stats, dgate, dpost_w, dbias, *(norm or ()))
+    B, L, D, g, mdt, ms, seed, pd = _post_norm_args("post_norm_residual_bwd", like, a, post_w, gate, keep,
+                                                    None if norm is None else (w, scale))
+    M = B * L
+    for t, n in zip(stats, ("post_mean", "post_rstd", "mean", "rstd") if norm is not None else ("post_mean", "post_rstd")):
+        if t is None or t.dtype != torch.float32 or t.numel() != M or not t.is_contiguous():
+            raise ValueError(f"post_norm_residual_bwd: {n} must be contiguous fp32 with {M} values")
+    if norm is not None and (dh.shape != a.shape or dh.dtype != a.dtype or not dh.is_contiguous() or x1.shape != a.shape
+                             or x1.dtype != torch.float32 or not x1.is_contiguous()):
+        raise ValueError("post_norm_residual_bwd: dh must be laid out like a, x1 contiguous fp32")
+    for t, n in ((dpost_w, "dpost_w"), (dbias, "dbias"), (dw, "dw")):
+        if t is not None and (t.shape != (D,) or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"post_norm_residual_bwd: {n} must be contiguous fp32 [{D}]")
+    for t, n in ((dgate, "dgate"), (dshift, "dshift"), (dscale, "dscale")):
+        if t is not None and (t.shape != (B, D) or t.dtype != torch.float32 or t.stride(1) != 1):
+            raise ValueError(f"post_norm_residual_bwd: {n} must be fp32 [{B}, {D}] with contiguous rows")
+    gs = dgate.stride(0) if dgate is not None else D
+    dms = dshift.stride(0) if dshift is not None else (dscale.stride(0) if dscale is not None else D)
+    if dshift is not None and dscale is not None and B > 1 and dscale.stride(0) != dms:
+        raise ValueError("post_norm_residual_bwd: dshift and dscale must share a row stride")
+    with _on_device(like):
+        dx, da = torch.empty_like(like), torch.empty_like(a)
+        if M == 0:
+            for t in (dgate, dshift, dscale):
+                if t is not None:
+                    t.zero_()
+            return dx, da
+        ws = torch.empty((6 if norm is not None else 3) * lib().sedd_ln_bwd_chunks(M, L) * D, dtype=torch.float32,
+                         device=like.device)
+        pm, pr, mean, rstd = tuple(stats) + (None,) * (4 - len(stats))
+        if norm is None:
+            mean = rstd = None
+        with _Timed("post_norm_residual_bwd", float(M) * D * (8 + 2 * a.element_size()
+                                                              + (0 if norm is None else 4 + a.element_size()))):
+            check(lib().sedd_post_norm_residual_bwd(_p(dx1), _p(dh), _p(x1), _p(w), _p(scale), _p(mean), _p(rstd), _p(a), _dt(a),
+                                                    _p(post_w), _p(g), mdt, ms, _p(pm), _p(pr), float(res_scale),
+                                                    float(inv_keep), seed, pd, _p(dx), _p(da), _p(ws), M, L, D, _stream()),
+                  "sedd_post_norm_residual_bwd")
+            check(lib().sedd_post_norm_residual_bwd_reduce(_p(ws), _p(dgate), gs, _p(dshift), _p(dscale), dms, _p(dpost_w),
+                                                           _p(dbias), _p(dw), M, L, D, _stream()),
+                  "sedd_post_norm_residual_bwd_reduce")
+    return dx, da
 
 
 def rotary_qkv_(qkv, cos, sin, conj=False):
@@ -1047,6 +1257,85 @@ def sumsq_clip(g, gscale=1.0, max_norm=0.0, ws=None, out=None):
 def clip_from_sumsq(out, gscale, max_norm):
     check(lib().sedd_clip_from_sumsq(_p(out), float(gscale), float(max_norm), _stream()), "sedd_clip_from_sumsq")
     return out
+
+
+def _dense(t):
+    """whether t's elements fill one stretch of memory, in whatever order of dimensions"""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if st != n:
+            return False
+        n *= sz
+    return True
+
+
+def _tensor_table(tensors, name):
+    """host arrays (addresses, sizes, dtypes) of a list of gradients, checked: one device, fp32 / bf16, dense, none of them
+    sharing memory with another."""
+    ptrs, sizes, kinds, spans = [], [], [], []
+    dev = tensors[0].device
+    for t in tensors:
+        if t.device != dev or dev.type != "cuda":
+            _one_device(name, tensors[0], t)
+        if t.is_sparse or not (t.is_contiguous() or _dense(t)):
+            raise ValueError(f"{name}: tensor of shape {tuple(t.shape)} and strides {tuple(t.stride())} is not dense")
+        p, n, k = t.data_ptr(), t.numel(), _dt(t)
+        ptrs.append(p)
+        sizes.append(n)
+        kinds.append(k)
+        if n:
+            spans.append((p, p + n * (2 if k == BF16 else 4)))
+    spans.sort()
+    end = 0
+    for lo, hi in spans:
+        if lo < end:
+            raise ValueError(f"{name}: two of the tensors share memory")
+        end = hi
+    n = len(ptrs)
+    return (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*kinds), n
+
+
+def _multi_norm(tab, max_norm, device):
+    n = tab[3]
+    # (allocated per call: two captured graphs, or two streams, never share it)
+    ws = torch.empty(4096 + n, dtype=torch.float64, device=device)
+    out = torch.empty(2, dtype=torch.float32, device=device)
+    check(lib().sedd_multi_norm_clip(tab[0], tab[1], tab[2], n, max_norm, _p(ws), ws.numel(), _p(out), _stream()),
+          "sedd_multi_norm_clip")
+    return out
+
+
+def grad_norm(grads):
+    """2-norm over all elements of a list of fp32 / bf16 tensors (squares summed in fp64) -> 0-dim fp32 tensor."""
+    grads = [grads] if torch.is_tensor(grads) else list(grads)
+    if not grads:
+        return torch.zeros(())
+    tab = _tensor_table(grads, "grad_norm")
+    with _on_device(grads[0]):
+        return _multi_norm(tab, 0.0, grads[0].device)[0]
+
+
+def clip_grad_norm_(grads, max_norm, error_if_nonfinite=False, round_coef=False):
+    """Scale a list of fp32 / bf16 gradient tensors in place by min(1, max_norm / (norm + 1e-6)), norm = their joint 2-norm
+    -> the norm before clipping, a 0-dim fp32 tensor on the device (not read on the host, except to raise under
+    error_if_nonfinite, before anything is scaled).  round_coef=True multiplies bf16 tensors by the coefficient as bf16 holds it
+    (off by up to 2^-9): bit parity with a loop of `grad.mul_(coef)`.  torch.nn.utils.clip_grad_norm_ on the gradients themselves (losses.py:65-66)."""
+    grads = [grads] if torch.is_tensor(grads) else list(grads)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_grad_norm_: max_norm must be >= 0, got {max_norm}")
+    if not grads:
+        return torch.zeros(())
+    tab = _tensor_table(grads, "clip_grad_norm_")
+    with _on_device(grads[0]):
+        out = _multi_norm(tab, max_norm, grads[0].device)
+        if error_if_nonfinite and not math.isfinite(float(out[0])):
+            raise RuntimeError(f"the norm of the gradients is {float(out[0])}: they were not clipped")
+        check(lib().sedd_multi_scale(tab[0], tab[1], tab[2], tab[3], out.data_ptr() + 4, 1 if round_coef else 0, _stream()),
+              "sedd_multi_scale")
+    return out[0]
 
 
 def adamw_ema_step(p, g, m, v, ema, p_bf16, clip_coef, grad_scale, lr, beta1, beta2, eps, weight_decay, step, ema_decay,

@@ -113,23 +113,57 @@ class AnalyticPredictor(Predictor):
         return sample_categorical(probs, u=u)
 
 
-class Denoiser:
-    """sampling.py:102-132"""
+@register_predictor(name="ancestral")
+class AncestralPredictor(Predictor):
+    """Ancestral update of the absorbing graph (not in the reference): a masked position leaves the mask with probability
+    (e^dsigma - 1) / (e^sigma - 1) = (m(t) - m(t - dt)) / m(t), m = 1 - e^-sigma, and its token is drawn from the model's
+    distribution over tokens, truncated by `truncation` (temperature / top_k / top_p / min_p) — one fused kernel.  Truncating
+    here shapes WHICH token appears, never WHEN a position is unmasked."""
+    truncation = {}
 
-    def __init__(self, graph, noise):
+    def update_fn(self, score_model, x, t, step_size, task=None, prot_indices=None, lig_indices=None, u=None):
+        sigma, nxt = self.noise(t)[0], self.noise(t - step_size)[0]
+        move = (torch.expm1(sigma - nxt) / torch.expm1(sigma)).reshape(-1)
+        log_score = model_log_score(score_model, x, sigma, task, prot_indices, lig_indices)
+        return self.graph.ancestral_step(log_score, x, move, u=u, **self.truncation)
+
+
+class Denoiser:
+    """sampling.py:102-132.  truncation: see AncestralPredictor; every position that is still masked then takes a token of
+    the truncated distribution."""
+
+    def __init__(self, graph, noise, truncation=None):
         self.graph = graph
         self.noise = noise
+        self.truncation = truncation
 
     def update_fn(self, score_model, x, t, step_size=None, task=None, prot_indices=None, lig_indices=None, u=None):
         sigma = self.noise(t)[0]
         log_score = model_log_score(score_model, x, sigma, task, prot_indices, lig_indices)
+        if self.truncation:
+            return self.graph.ancestral_step(log_score, x, u=u, **self.truncation)
         return self.graph.predictor_step(_L.STEP_DENOISE, log_score, x, sigma, u=u)
 
 
 def get_sampling_fn(config, graph, noise, batch_dims, eps, device):
-    """sampling.py:135-146"""
+    """sampling.py:135-146; config.sampling may also hold temperature / top_k / top_p / min_p (get_pc_sampler)."""
+    cut = {k: getattr(config.sampling, k) for k in ("temperature", "top_k", "top_p", "min_p")
+           if getattr(config.sampling, k, None) is not None}
     return get_pc_sampler(graph=graph, noise=noise, batch_dims=batch_dims, predictor=config.sampling.predictor,
-                          steps=config.sampling.steps, denoise=config.sampling.noise_removal, eps=eps, device=device)
+                          steps=config.sampling.steps, denoise=config.sampling.noise_removal, eps=eps, device=device, **cut)
+
+
+def _truncation(predictor, graph, temperature, top_k, top_p, min_p):
+    """the truncation that was asked for, or {} for none; refuses what cannot honour it"""
+    cut = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    if not any(torch.is_tensor(v) for v in cut.values()) and (temperature, top_k, top_p, min_p) == (1.0, 0, 1.0, 0.0):
+        return {}
+    if predictor not in ("ancestral", "none"):
+        raise ValueError(f"temperature / top_k / top_p / min_p need predictor='ancestral' (or 'none'), got {predictor!r}: the "
+                         "Euler and Analytic updates mix the mask state into the distribution that would be truncated")
+    if not hasattr(graph, "ancestral_step"):
+        raise ValueError("temperature / top_k / top_p / min_p need the absorbing graph")
+    return cut
 
 
 class _GraphedStep:
@@ -169,15 +203,22 @@ class _GraphedStep:
 
 
 def get_pc_sampler(graph, noise, batch_dims, predictor, steps, denoise=True, eps=1e-5, device=torch.device('cpu'),
-                   proj_fun=lambda x: x, hip_graph=False):
-    """sampling.py:149-175.  hip_graph=True (not in the reference): the predictor update is captured once per (model,
+                   proj_fun=lambda x: x, hip_graph=False, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """sampling.py:149-175.  temperature / top_k / top_p / min_p (not in the reference; predictor "ancestral", or "none" for
+    one-shot denoising, absorbing graph): numbers, or device tensors with one value per sequence — the tokens that appear are
+    drawn from the truncated distribution (ops.sample_truncated).  hip_graph=True (not in the reference): the predictor update is captured once per (model,
     task, conditioning, noise form) as a HIP graph and replayed `steps` times — same kernels, same tokens for the same
     noise; for launch-bound (small) models.  It needs proj_fun and the model's forward to be capturable (device-side
     work only) and takes noise_seq as explicit tensors or None (torch's generator), not as a PhiloxStream (whose offsets
     are host integers)."""
+    truncation = _truncation(predictor, graph, temperature, top_k, top_p, min_p)
+    if predictor == "ancestral" and not hasattr(graph, "ancestral_step"):
+        raise ValueError("predictor 'ancestral' needs the absorbing graph")
     predictor = get_predictor(predictor)(graph, noise)
+    if truncation and isinstance(predictor, AncestralPredictor):
+        predictor.truncation = truncation
     projector = proj_fun
-    denoiser = Denoiser(graph, noise)
+    denoiser = Denoiser(graph, noise, truncation)
     graphed = {}
 
     @torch.no_grad()
