@@ -279,7 +279,8 @@ def _run_norm(s):
 def _run_clip(s):
     if own:
         from protein_lig_sedd_amd import ops
-        norm = ops.clip_grad_norm_(s["grads"], s["case"]["max_norm"])
+        # (the coefficient as each tensor's type holds it, as in the plain form's mul_)
+        norm = ops.clip_grad_norm_(s["grads"], s["case"]["max_norm"], round_coef=True)
     else:
         norm = _clip_plain(s["grads"], s["case"]["max_norm"])
     return {"norm": norm, "grads": s["arenas"]}
