@@ -196,6 +196,187 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, do
     }
 }
 
+// ------------------------------------------------------------------------------------------- the same in 32 bits
+// Per row the 32-bit pass either settles the decision or gives the row up to resolve_row64.  What its quantities are off by
+// (v_exp_f32, v_log_f32 and v_rcp_f32 measured below 2^-23 relative):
+//   q_j: d2 = (x - max) * (log2 e / T) has four roundings, so q_j is off by |d2| 4 2^-24 ln 2 + 2^-23 relative.
+//   q_j / E_j: a winner has q_j >= (1 / 23.1) * 1e-10, the smallest E over the largest (the first of the order has q = 1), so
+//     |d2| <= 39 and the ratio is off by 7.2e-6; two of them are told apart when they differ by more than 1.45e-5: RATIO_TOL.
+//   S, W: sum q |d2| <= W log2 V, so a sum is off by (log2 V * 2.8 + 2) 2^-24 W and by its n adds one after the other, n 2^-24 W:
+//     V <= 64 in one lane 5.0e-6 W; 64 a lane and 10 across, V = 32768: 7.1e-6 W.  S against P W: 1.42e-5 W at most: MASS_TOL.
+// A comparison nearer than that, and every row whose maximum or temperature leaves the range of these bounds, is "near".
+#define RATIO_TOL 0x1p-15f
+#define MASS_TOL 0x1p-15f
+#define LOG2E 1.44269504f
+#define LN2 0.693147181f
+
+__device__ __forceinline__ float inv_noise(float u) {  // 1 / E
+    const float l2 = __builtin_amdgcn_logf(noise_arg(u));
+    return __builtin_amdgcn_rcpf(__builtin_fmaf(-LN2, l2, 1e-10f));
+}
+// log2(e) / T, and whether T lies where the bounds hold
+__device__ __forceinline__ float rate_of(float T, bool& near) {
+    near = near || !(T > 1e-30f && T < 1e30f);
+    return LOG2E / T;
+}
+// a number on the key scale back as the float it stands for
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
+}
+enum Verdict { KEPT, DROPPED, NEAR };
+// what the 32-bit numbers say about the entry of a given rank, mass before it and weight
+__device__ __forceinline__ Verdict judge(const RowParams& rp, int rank, float S, float W, float q, float best, float second) {
+    if (rank != 0) {
+        const float margin = rp.P * W - S, tol = MASS_TOL * W;
+        if (rank >= rp.k || (rp.P < 1.f && margin < -tol) || q < rp.m * (1.f - RATIO_TOL)) return DROPPED;
+        if ((rp.P < 1.f && !(margin > tol)) || (rp.m > 0.f && !(q > rp.m * (1.f + RATIO_TOL)))) return NEAR;
+    }
+    return second < best * (1.f - RATIO_TOL) ? KEPT : NEAR;
+}
+
+// ---- V <= 64: a lane owns a row.  Everything is register arithmetic over the lane's own entries, no cross-lane traffic; the
+// rows of a wave are neighbours in memory, so the loads of a wave cover one stretch of it.  In the middle of a sampler run most
+// rows are not sampled: a block packs those that are to its first lanes, and the waves behind them end.
+template <typename T, int VP> __device__ __forceinline__ void load_entries(const T* p, int V, float (&x)[VP]) {
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < VP; c += E) {
+        if (c + E <= VP && c + E <= V) {
+            struct __attribute__((packed)) { T e[E]; } v;
+            __builtin_memcpy(&v, p + c, 16);
+#pragma unroll
+            for (int i = 0; i < E; ++i) if (c + i < VP) x[c + i] = to_f32<T>(v.e[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (c + i < VP) x[c + i] = c + i < V ? to_f32<T>(p[c + i]) : -INFINITY;
+        }
+    }
+}
+
+template <typename T, int VP>
+__global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
+    __shared__ int s_cnt;
+    __shared__ uint8_t s_list[256];
+    const int64_t row0 = (int64_t)blockIdx.x * 256, b0 = row0 / a.L, off0 = row0 - b0 * a.L;
+    const int V = a.V, lane = threadIdx.x & 63;
+    int r = threadIdx.x;
+    bool on = row0 + r < a.M;
+    auto batch_of = [&](int rr) -> int64_t {
+        const int64_t q = off0 + rr;
+        return a.L >= 256 ? b0 + (q >= a.L) : b0 + (uint32_t)q / (uint32_t)a.L;
+    };
+    if (a.xcur) {  // (uniform: the barriers are met by the whole block)
+        if (threadIdx.x == 0) s_cnt = 0;
+        __syncthreads();
+        bool go = false;
+        if (on) {
+            go = row_moves(a, row0 + r, a.move ? batch_of(r) : 0);
+            if (!go) a.out[row0 + r] = a.xcur[row0 + r];
+        }
+        const unsigned long long mask = __ballot(go);
+        int base = 0;
+        if (lane == 0 && mask) base = atomicAdd(&s_cnt, __popcll(mask));
+        base = __shfl(base, 0, 64);
+        if (go) s_list[base + __popcll(mask & ((1ull << lane) - 1ull))] = (uint8_t)r;
+        __syncthreads();
+        on = (int)threadIdx.x < s_cnt;
+        r = on ? s_list[threadIdx.x] : 0;
+    }
+    if (!__ballot(on)) return;
+    const int64_t row = on ? row0 + r : row0, b = batch_of(on ? r : 0);
+    const RowParams rp = row_params(a, b);
+    float x[VP], ie[VP];
+    load_entries<T, VP>((const T*)a.x + row * a.ld, V, x);
+    load_entries<float, VP>(a.u + row * a.ldu, V, ie);
+    float mx = -INFINITY;
+    int mi = 0;
+#pragma unroll
+    for (int j = 0; j < VP; ++j) {
+        x[j] = x[j] > -INFINITY ? x[j] : -INFINITY;  // (NaN is no candidate)
+        mi = x[j] > mx ? j : mi;
+        mx = fmaxf(mx, x[j]);
+    }
+    int got = -1;  // < 0: open;  the row's answer otherwise
+    bool near = mx == INFINITY, open = on && mx > -INFINITY;
+    const bool empty = !(mx > -INFINITY);
+    if (!(rp.T > 0.f)) { got = mi; open = false; }
+    const float c = rate_of(rp.T, near);
+    near = near && open;
+    open = open && !near;
+    float b1 = -1.f, b2 = -1.f, xw = 0.f, W = 0.f;
+    int iw = 0;
+#pragma unroll
+    for (int j = 0; j < VP; ++j) {
+        const float q = __builtin_amdgcn_exp2f((x[j] - mx) * c);
+        W += q;
+        ie[j] = x[j] > -INFINITY ? q * inv_noise(ie[j]) : -1.f;  // the ratio takes the noise's place
+        b2 = __builtin_amdgcn_fmed3f(b1, b2, ie[j]);
+        iw = ie[j] > b1 ? j : iw;
+        xw = ie[j] > b1 ? x[j] : xw;
+        b1 = fmaxf(b1, ie[j]);
+    }
+    if (__ballot(open && rp.k < V && rp.P < 1.f)) {  // mass of the k first: the k-th largest value, bit by bit
+        uint32_t t = 0;
+        constexpr int LOW = sizeof(T) == 2 ? 16 : 0;
+        bool exact = false;  // exactly k entries at or above t: lower bits change nothing
+        for (int bit = 31; bit >= LOW; --bit) {
+            const uint32_t ct = t | (1u << bit);
+            const float tv = key_value(ct);
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < VP; ++j) n += x[j] >= tv;
+            if (!exact && n >= rp.k) { t = ct; exact = n == rp.k; }
+            if (!__ballot(open && !exact)) break;
+        }
+        const float tv = key_value(t);
+        float s = 0.f;
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < VP; ++j) {
+            const float q = __builtin_amdgcn_exp2f((x[j] - mx) * c);
+            s += ((x[j] > tv) | (exact & (x[j] == tv))) ? q : 0.f;
+            n += x[j] > tv;
+        }
+        if (t && rp.k < V) W = exact ? s : s + (float)(rp.k - n) * __builtin_amdgcn_exp2f((tv - mx) * c);
+    }
+    if (open && rp.k >= V && !(rp.P < 1.f) && !(rp.m > 0.f)) {  // nothing is cut off
+        if (b2 < b1 * (1.f - RATIO_TOL)) got = iw;
+        else near = true;
+        open = false;
+    }
+    while (__ballot(open)) {
+        float S = 0.f, n1 = -1.f, n2 = -1.f, nx = 0.f;
+        int rank = 0, ni = 0;
+#pragma unroll
+        for (int j = 0; j < VP; ++j) {
+            const bool before = (x[j] > xw) | ((x[j] == xw) & (j < iw));
+            const float q = __builtin_amdgcn_exp2f((x[j] - mx) * c), v = before ? ie[j] : -1.f;
+            S += before ? q : 0.f;
+            rank += before;
+            n2 = __builtin_amdgcn_fmed3f(n1, n2, v);
+            ni = v > n1 ? j : ni;
+            nx = v > n1 ? x[j] : nx;
+            n1 = fmaxf(n1, v);
+        }
+        const Verdict w = judge(rp, rank, S, W, __builtin_amdgcn_exp2f((xw - mx) * c), b1, b2);
+        if (open && w != DROPPED) {
+            open = false;
+            if (w == KEPT) got = iw;
+            else near = true;
+        }
+        b1 = n1; b2 = n2; iw = ni; xw = nx;
+    }
+    int64_t ans = empty ? row_empty(a) : (int64_t)got;
+    for (unsigned long long todo = __ballot(near); todo; todo &= todo - 1) {
+        const int src = __builtin_ctzll(todo);
+        const int rr = __builtin_amdgcn_readlane(on ? r : 0, src);
+        const int64_t v = resolve_row64<T, 64>(a, row0 + rr, batch_of(rr), nullptr, nullptr);
+        if (lane == src) ans = v;
+    }
+    if (on) a.out[row] = ans;
+}
+
 template <typename T, int NT>
 __global__ void __launch_bounds__(256) sample_row64_kernel(SampleArgs a) {
     __shared__ double sd[4];
@@ -210,8 +391,23 @@ __global__ void __launch_bounds__(256) sample_row64_kernel(SampleArgs a) {
     }
 }
 
+template <typename T, int VP> static void launch_lane(const SampleArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((sample_lane_kernel<T, VP>), dim3((unsigned)((a.M + 255) / 256)), dim3(256), 0, st, a);
+}
 template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t st) {
-    if (a.V <= 4096)
+    // V up to a multiple of 4 (8 above 32): the entries behind V cost arithmetic, and a row is never read past its end
+    if (a.V <= 4) launch_lane<T, 4>(a, st);
+    else if (a.V <= 8) launch_lane<T, 8>(a, st);
+    else if (a.V <= 12) launch_lane<T, 12>(a, st);
+    else if (a.V <= 16) launch_lane<T, 16>(a, st);
+    else if (a.V <= 20) launch_lane<T, 20>(a, st);
+    else if (a.V <= 24) launch_lane<T, 24>(a, st);
+    else if (a.V <= 28) launch_lane<T, 28>(a, st);
+    else if (a.V <= 32) launch_lane<T, 32>(a, st);
+    else if (a.V <= 40) launch_lane<T, 40>(a, st);
+    else if (a.V <= 48) launch_lane<T, 48>(a, st);
+    else if (a.V <= 64) launch_lane<T, 64>(a, st);
+    else if (a.V <= 4096)
         hipLaunchKernelGGL((sample_row64_kernel<T, 64>), dim3(sedd_grid_for(a.M, 4, 256 * 8)), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((sample_row64_kernel<T, 256>), dim3(sedd_grid_for(a.M, 1, 256 * 8)), dim3(256), 0, st, a);
