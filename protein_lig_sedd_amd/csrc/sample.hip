@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     return v > -INFINITY ? key : 0u;
 }
 // u + 1e-10 in 32 bits as the reference's catsample rounds it, kept inside (0, 1] whatever u is
-__device__ __forceinline__ float noise_arg(float u) { return fminf(fmaxf(u + 1e-10f, 1e-10f), 1.0f); }
+__device__ __forceinline__ float noise_arg(float u) { return __builtin_amdgcn_fmed3f(u + 1e-10f, 1e-10f, 1.0f); }
 
 // ------------------------------------------------------------------------------- the definition itself, in 64 bits
 // NT threads (a power of two of whole waves) work one row together, reading it from memory in every pass.
@@ -223,6 +223,10 @@ __device__ __forceinline__ float rate_of(float T, bool& near) {
 __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
 }
+// a key found down to bit LOW, completed: below zero the order turns the bits round, and a bf16 value's low half is all ones there
+template <int LOW> __device__ __forceinline__ uint32_t whole_key(uint32_t t) {
+    return t && !(t >> 31) ? t | ((1u << LOW) - 1u) : t;
+}
 enum Verdict { KEPT, DROPPED, NEAR };
 // what the 32-bit numbers say about the entry of a given rank, mass before it and weight
 __device__ __forceinline__ Verdict judge(const RowParams& rp, int rank, float S, float W, float q, float best, float second) {
@@ -329,6 +333,7 @@ __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
             if (!exact && n >= rp.k) { t = ct; exact = n == rp.k; }
             if (!__ballot(open && !exact)) break;
         }
+        t = whole_key<LOW>(t);
         const float tv = key_value(t);
         float s = 0.f;
         int n = 0;
@@ -377,22 +382,387 @@ __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
     if (on) a.out[row] = ans;
 }
 
+// ---- V > 64: NW waves own a row, its entries in registers (NE per lane, four neighbours at a time).
+// Sums and maxima across a wave go through DPP adds (four steps inside rows of 16 lanes, two across them).
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_f(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ float dpp_sum(float v) {
+    v += dpp_f<0x111, 0xf>(0.f, v);
+    v += dpp_f<0x112, 0xf>(0.f, v);
+    v += dpp_f<0x114, 0xf>(0.f, v);
+    v += dpp_f<0x118, 0xf>(0.f, v);
+    v += dpp_f<0x142, 0xa>(0.f, v);
+    v += dpp_f<0x143, 0xc>(0.f, v);
+    return lane63(v);
+}
+__device__ __forceinline__ float dpp_max(float v) {
+    v = fmaxf(v, dpp_f<0x111, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x112, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x114, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x118, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp_f<0x143, 0xc>(v, v));
+    return lane63(v);
+}
+// the best and second best ratio, with the best one's value and index
+struct Best {
+    float b1, b2, x;
+    int i;
+};
+// one lane's numbers joined over the NW waves of a row; every member is called by all of them.  The exchange alternates
+// between two buffers, so a barrier per call is enough: a buffer is written again two calls later.
+template <int NW> struct RowRed {
+    float (*buf)[6 * NW];
+    int turn = 0;
+    __device__ __forceinline__ float max(float v) {
+        v = dpp_max(v);
+        if constexpr (NW > 1) {
+            float* o = swap();
+            if ((threadIdx.x & 63) == 0) o[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = dpp_max(o[threadIdx.x & (NW - 1)]);
+        }
+        return v;
+    }
+    __device__ __forceinline__ float sum(float v) {
+        v = dpp_sum(v);
+        if constexpr (NW > 1) {
+            float* o = swap();
+            if ((threadIdx.x & 63) == 0) o[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = dpp_sum((threadIdx.x & 63) < NW ? o[threadIdx.x & (NW - 1)] : 0.f);
+        }
+        return v;
+    }
+    __device__ __forceinline__ int count(int n) {  // n is the wave's own (the same in all lanes)
+        if constexpr (NW > 1) {
+            float* o = swap();
+            if ((threadIdx.x & 63) == 0) o[threadIdx.x >> 6] = (float)n;  // (below 2^24)
+            __syncthreads();
+            n = (int)dpp_sum((threadIdx.x & 63) < NW ? o[threadIdx.x & (NW - 1)] : 0.f);
+        }
+        return n;
+    }
+    // joins `v`, and the sum and the count beside it
+    __device__ __forceinline__ void join(Best& v, float& s, int& n) {
+        pick(v, 64);
+        s = dpp_sum(s);
+        if constexpr (NW > 1) {
+            float* o = swap();
+            const int w = threadIdx.x >> 6, l = threadIdx.x & (NW - 1);
+            if ((threadIdx.x & 63) == 0) {
+                o[w] = v.b1; o[NW + w] = v.b2; o[2 * NW + w] = v.x; o[3 * NW + w] = __int_as_float(v.i);
+                o[4 * NW + w] = s; o[5 * NW + w] = (float)n;
+            }
+            __syncthreads();
+            v = {o[l], o[NW + l], o[2 * NW + l], __float_as_int(o[3 * NW + l])};
+            const bool mine = (threadIdx.x & 63) < NW;
+            s = dpp_sum(mine ? o[4 * NW + l] : 0.f);
+            n = (int)dpp_sum(mine ? o[5 * NW + l] : 0.f);
+            pick(v, NW);
+        }
+    }
+
+  private:
+    __device__ __forceinline__ float* swap() { turn ^= 1; return buf[turn]; }
+    // the best of `n` different lanes (the wave holds them 64 / n times over).  Of equals any will do: the row is then near
+    __device__ __forceinline__ void pick(Best& v, int n) {
+        const float top = dpp_max(v.b1);
+        const int src = __builtin_ctzll(__ballot(v.b1 == top));
+        const bool won = ((int)(threadIdx.x & 63) & (n - 1)) == (src & (n - 1));
+        const float second = dpp_max(won ? v.b2 : v.b1);
+        v.x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v.x), src));
+        v.i = __builtin_amdgcn_readlane(v.i, src);
+        v.b1 = top;
+        v.b2 = second;
+    }
+};
+// the largest key t with at least k entries at or above it (0: there are not so many), bit by bit down to LOW; exactly k
+// entries above a key end the search early.  Counts are popcounts of compare masks: no arithmetic across lanes.
+template <int LOW, int N, class R> __device__ __forceinline__ uint32_t kth_key(const float (&x)[N], int k, R& red) {
+    uint32_t t = 0;
+    for (int bit = 31; bit >= LOW; --bit) {
+        const uint32_t ct = t | (1u << bit);
+        const float tv = key_value(ct);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += __popcll(__ballot(x[i] >= tv));
+        n = red.count(n);
+        if (n >= k) {
+            t = ct;
+            if (n == k) break;
+        }
+    }
+    return whole_key<LOW>(t);
+}
+// mass of the k first, where t is their kth_key
+template <int N, class R>
+__device__ __forceinline__ float mass_of_first(const float (&x)[N], int k, uint32_t t, float mx, float c, R& red) {
+    const float tv = key_value(t);
+    float s = 0.f;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        s += x[i] > tv ? __builtin_amdgcn_exp2f((x[i] - mx) * c) : 0.f;
+        n += __popcll(__ballot(x[i] > tv));
+    }
+    s = red.sum(s);
+    n = red.count(n);
+    // the rest of the k lie at tv, or — where the search ended early — between tv and the next entry above it
+    float at = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) at = fmaxf(at, x[i] == tv ? x[i] : -INFINITY);
+    at = red.max(at);
+    return at > -INFINITY ? s + (float)(k - n) * __builtin_amdgcn_exp2f((tv - mx) * c) : s;
+}
+// the elimination over entries (x[i], index jof(i)) with ratios r[i] (-1: no candidate)
+template <int N, class R, class J>
+__device__ __forceinline__ int eliminate(const RowParams& rp, bool cut, const float (&x)[N], const float (&r)[N], J jof,
+                                         float mx, float c, float W, R& red, bool& near) {
+    Best v{-1.f, -1.f, 0.f, 0};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v.b2 = __builtin_amdgcn_fmed3f(v.b1, v.b2, r[i]);
+        v.i = r[i] > v.b1 ? i : v.i;
+        v.x = r[i] > v.b1 ? x[i] : v.x;
+        v.b1 = fmaxf(v.b1, r[i]);
+    }
+    v.i = jof(v.i);
+    float s = 0.f;
+    int rank = 0;
+    red.join(v, s, rank);
+    if (!cut) {
+        near = !(v.b2 < v.b1 * (1.f - RATIO_TOL));
+        return v.i;
+    }
+    for (;;) {
+        Best w{-1.f, -1.f, 0.f, 0};
+        s = 0.f;
+        rank = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool before = (x[i] > v.x) | ((x[i] == v.x) & (jof(i) < v.i));
+            const float q = __builtin_amdgcn_exp2f((x[i] - mx) * c), ri = before ? r[i] : -1.f;
+            s += before ? q : 0.f;
+            rank += __popcll(__ballot(before));
+            w.b2 = __builtin_amdgcn_fmed3f(w.b1, w.b2, ri);
+            w.i = ri > w.b1 ? i : w.i;
+            w.x = ri > w.b1 ? x[i] : w.x;
+            w.b1 = fmaxf(w.b1, ri);
+        }
+        w.i = jof(w.i);
+        red.join(w, s, rank);
+        const Verdict d = judge(rp, rank, s, W, __builtin_amdgcn_exp2f((v.x - mx) * c), v.b1, v.b2);
+        if (d != DROPPED) {
+            near = d == NEAR;
+            return v.i;
+        }
+        v = w;
+    }
+}
+
+// Where top-k or min-p leaves few entries, they are packed, four to a lane of one wave, and only their noise is read:
+// the k-th largest of the lanes' own maxima is a bound that at least k entries reach (k distinct lanes), usually not many more.
+#define PACK 256
+template <typename T, int NW, int NE>
+__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64) sample_wide_kernel(SampleArgs a) {
+    constexpr int NT = NW * 64, ROWS = NW == 1 ? 4 : 1, LOW = sizeof(T) == 2 ? 16 : 0;
+    __shared__ float s_x[ROWS][PACK];
+    __shared__ int s_j[ROWS][PACK];
+    __shared__ float s_red[2][6 * NW];
+    __shared__ double s_d[NW];
+    __shared__ int64_t s_i[NW];
+    __shared__ int s_n, s_ans, s_near;
+    const int V = a.V, lane = threadIdx.x & 63, tid = NW == 1 ? lane : (int)threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = NW == 1 ? wave : 0;
+    RowRed<NW> red{s_red};
+    RowRed<1> alone{nullptr};
+    auto jof = [&](int i) { return (i >> 2) * (4 * NT) + tid * 4 + (i & 3); };
+    // (One row per wave and launch, no loop: out of one, the constants of the 64-bit exp and log would be hoisted and kept in
+    // a hundred registers.)
+    const int64_t row = (int64_t)blockIdx.x * ROWS + slot;
+    {
+        if (row >= a.M) return;
+        const int64_t b = row / a.L;
+        if (!row_moves(a, row, b)) {
+            if (tid == 0) a.out[row] = a.xcur[row];
+            return;
+        }
+        RowParams rp = row_params(a, b);
+        const T* px = (const T*)a.x + row * a.ld;
+        const float* pu = a.u + row * a.ldu;
+        float x[NE], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NE; i += 4) {
+            const int j = jof(i);
+            if (j + 4 <= V) {
+                struct __attribute__((packed)) { T e[4]; } v;
+                __builtin_memcpy(&v, px + j, 4 * sizeof(T));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i + k] = to_f32<T>(v.e[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i + k] = j + k < V ? to_f32<T>(px[j + k]) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;
+            top = fmaxf(top, x[i]);
+        }
+        const float mx = red.max(top);
+        if (!(mx > -INFINITY)) {
+            if (tid == 0) a.out[row] = row_empty(a);
+            return;
+        }
+        bool near = mx == INFINITY;
+        int got = -1;
+        if (!(rp.T > 0.f)) {
+            float first = -INFINITY;  // (an index is below 2^24)
+#pragma unroll
+            for (int i = NE - 1; i >= 0; --i) first = x[i] == mx ? -(float)jof(i) : first;
+            got = (int)-red.max(first);
+            near = false;
+        } else {
+            const float c = rate_of(rp.T, near);
+            if (!near) {
+                // a bound that what is kept reaches
+                float thr = -INFINITY;
+                uint32_t t = 0;
+                int n = PACK + 1;
+                auto reach = [&]() __attribute__((always_inline)) {
+                    int m = 0;
+#pragma unroll
+                    for (int i = 0; i < NE; ++i) m += __popcll(__ballot((x[i] >= thr) & (x[i] > -INFINITY)));
+                    return m;
+                };
+                if (rp.k < V) {
+                    if (rp.k <= PACK && rp.k <= NT) {
+                        const float lm[1] = {top};
+                        const uint32_t bound = kth_key<LOW>(lm, rp.k, red);
+                        if (bound) {
+                            thr = key_value(bound);
+                            n = red.count(reach());
+                        }
+                    }
+                    if (n > PACK) {
+                        t = kth_key<LOW>(x, rp.k, red);
+                        if (t) thr = key_value(t);
+                        else rp.k = V;  // (fewer candidates than k)
+                        n = red.count(reach());
+                    }
+                } else if (!(rp.P < 1.f) && rp.m > 0.f) {
+                    thr = mx + (__builtin_amdgcn_logf(rp.m) - 0.01f) / c;
+                    n = red.count(reach());
+                }
+                const bool cut = rp.k < V || rp.P < 1.f || rp.m > 0.f;
+                if (n <= PACK && (rp.k < V || !(rp.P < 1.f))) {
+                    int base = 0;
+                    if constexpr (NW > 1) {
+                        if (threadIdx.x == 0) s_n = 0;
+                        __syncthreads();
+                        const int mine = reach();
+                        if (lane == 0) base = atomicAdd(&s_n, mine);  // (the order of the packed entries does not matter)
+                        base = __builtin_amdgcn_readfirstlane(base);
+                    }
+#pragma unroll
+                    for (int i = 0; i < NE; ++i) {
+                        const bool in = (x[i] >= thr) & (x[i] > -INFINITY);
+                        const unsigned long long mask = __ballot(in);
+                        if (in) {
+                            const int at = base + __popcll(mask & ((1ull << lane) - 1ull));
+                            s_x[slot][at] = x[i];
+                            s_j[slot][at] = jof(i);
+                        }
+                        base += __popcll(mask);
+                    }
+                    if constexpr (NW > 1) __syncthreads();
+                    else __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
+                    if (NW == 1 || wave == 0) {
+                        float y[4], r[4];
+                        int jj[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int e = lane + 64 * i;
+                            y[i] = e < n ? s_x[slot][e] : -INFINITY;
+                            jj[i] = e < n ? s_j[slot][e] : 0;
+                            r[i] = e < n ? __builtin_amdgcn_exp2f((y[i] - mx) * c) * inv_noise(pu[jj[i]]) : -1.f;
+                        }
+                        float W = 0.f;
+                        if (rp.P < 1.f) {
+                            if (!t) t = kth_key<LOW>(y, rp.k, alone);
+                            W = mass_of_first(y, rp.k, t, mx, c, alone);
+                        }
+                        got = eliminate<4>(rp, cut, y, r, [&](int i) { return i == 0 ? jj[0] : i == 1 ? jj[1] : i == 2 ? jj[2] : jj[3]; },
+                                           mx, c, W, alone, near);
+                        if constexpr (NW > 1) {
+                            if (lane == 0) { s_ans = got; s_near = near; }
+                        }
+                    }
+                    if constexpr (NW > 1) {
+                        __syncthreads();
+                        got = s_ans;
+                        near = s_near != 0;
+                    } else {
+                        __builtin_amdgcn_wave_barrier();
+                    }
+                } else {
+                    float r[NE], W = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NE; i += 4) {
+                        const int j = jof(i);
+                        float u4[4];
+                        if (j + 4 <= V) {
+                            struct __attribute__((packed)) { float e[4]; } v;
+                            __builtin_memcpy(&v, pu + j, 16);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) u4[k] = v.e[k];
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) u4[k] = j + k < V ? pu[j + k] : 0.5f;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float q = __builtin_amdgcn_exp2f((x[i + k] - mx) * c);
+                            W += q;
+                            r[i + k] = ((x[i + k] >= thr) & (x[i + k] > -INFINITY)) ? q * inv_noise(u4[k]) : -1.f;
+                        }
+                    }
+                    if (rp.P < 1.f) W = t ? mass_of_first(x, rp.k, t, mx, c, red) : red.sum(W);
+                    got = eliminate<NE>(rp, cut, x, r, jof, mx, c, W, red, near);
+                }
+            }
+        }
+        int64_t ans = got;
+        if (near) {
+            if constexpr (NW > 1) __syncthreads();
+            ans = resolve_row64<T, NT>(a, row, b, s_d, s_i);
+        }
+        if (tid == 0) a.out[row] = ans;
+    }
+}
+
 template <typename T, int NT>
-__global__ void __launch_bounds__(256) sample_row64_kernel(SampleArgs a) {
-    __shared__ double sd[4];
-    __shared__ int64_t si[4];
-    const int64_t stride = (int64_t)gridDim.x * (256 / NT);
-    for (int64_t row = (int64_t)blockIdx.x * (256 / NT) + threadIdx.x / NT; row < a.M; row += stride) {
+__global__ void __launch_bounds__(NT) sample_row64_kernel(SampleArgs a) {
+    __shared__ double sd[NT / 64];
+    __shared__ int64_t si[NT / 64];
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const int64_t b = row / a.L;
         int64_t got;
         if (!row_moves(a, row, b)) got = a.xcur[row];
         else got = resolve_row64<T, NT>(a, row, b, sd, si);
-        if ((threadIdx.x & (NT - 1)) == 0) a.out[row] = got;
+        if (threadIdx.x == 0) a.out[row] = got;
     }
 }
 
 template <typename T, int VP> static void launch_lane(const SampleArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((sample_lane_kernel<T, VP>), dim3((unsigned)((a.M + 255) / 256)), dim3(256), 0, st, a);
+}
+template <typename T, int NW, int NE> static void launch_wide(const SampleArgs& a, hipStream_t st) {
+    constexpr int R = NW == 1 ? 4 : 1;
+    hipLaunchKernelGGL((sample_wide_kernel<T, NW, NE>), dim3((unsigned)((a.M + R - 1) / R)), dim3(NW == 1 ? 256 : NW * 64), 0, st, a);
 }
 template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t st) {
     // V up to a multiple of 4 (8 above 32): the entries behind V cost arithmetic, and a row is never read past its end
@@ -407,10 +777,18 @@ template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t
     else if (a.V <= 40) launch_lane<T, 40>(a, st);
     else if (a.V <= 48) launch_lane<T, 48>(a, st);
     else if (a.V <= 64) launch_lane<T, 64>(a, st);
-    else if (a.V <= 4096)
-        hipLaunchKernelGGL((sample_row64_kernel<T, 64>), dim3(sedd_grid_for(a.M, 4, 256 * 8)), dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((sample_row64_kernel<T, 256>), dim3(sedd_grid_for(a.M, 1, 256 * 8)), dim3(256), 0, st, a);
+    // a wave per row while its entries fit 64 a lane, four waves up to 16384, sixteen up to 32768 (32 a lane: such a block has
+    // 128 registers a lane)
+    else if (a.V <= 256) launch_wide<T, 1, 4>(a, st);
+    else if (a.V <= 512) launch_wide<T, 1, 8>(a, st);
+    else if (a.V <= 1024) launch_wide<T, 1, 16>(a, st);
+    else if (a.V <= 2048) launch_wide<T, 1, 32>(a, st);
+    else if (a.V <= 48 * 64) launch_wide<T, 1, 48>(a, st);
+    else if (a.V <= 4096) launch_wide<T, 1, 64>(a, st);
+    else if (a.V <= 8192) launch_wide<T, 4, 32>(a, st);
+    else if (a.V <= 16384) launch_wide<T, 4, 64>(a, st);
+    else if (a.V <= 32768) launch_wide<T, 16, 32>(a, st);
+    else hipLaunchKernelGGL((sample_row64_kernel<T, 1024>), dim3(sedd_grid_for(a.M, 1, 512)), dim3(1024), 0, st, a);
 }
 
 extern "C" int sedd_sample_truncated(const void* logits, int dtype, int64_t ld, const float* u, int64_t ldu,

@@ -103,6 +103,12 @@ def test_ties_and_equal_rows(V):
     for x in (torch.zeros(64, V), torch.randint(0, 3, (64, V), generator=g).float(), torch.full((64, V), -7.25)):
         for c in (dict(), dict(top_p=0.5), dict(top_p=0.25, top_k=4), dict(top_k=3), dict(min_p=1.0), dict(top_p=1e-6)):
             check(x.to(DEV), u, **c)
+    for dtype in (torch.float32, torch.bfloat16):  # equal scores across the border of the k, above and below zero
+        x = torch.randint(-5, 4, (96, V), generator=g).to(dtype).to(DEV) * 0.75
+        uu = torch.rand(96, V, generator=g).to(DEV)
+        for k in (2, 3, 5, max(V // 3, 1), max(V - 2, 1)):
+            for P in (0.3, 0.6, 0.9):
+                check(x, uu, top_k=k, top_p=P)
     x = torch.zeros(8, V)
     x[:, V // 2:] = -0.0  # both zeros are one value
     check(x.to(DEV), u[:8], top_k=max(V // 2, 1), top_p=0.9)
