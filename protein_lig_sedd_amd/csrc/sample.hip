@@ -46,6 +46,13 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& a, int64_t b) 
     if (r.k <= 0 || r.k > a.V) r.k = a.V;
     return r;
 }
+// batch element of a row (0 where no parameter goes by it): in 32 bits where the rows allow, a 64-bit division is hundreds of
+// instructions
+__device__ __forceinline__ int64_t batch_of_row(const SampleArgs& a, int64_t row) {
+    if (!a.T && !a.P && !a.m && !a.k && !a.move) return 0;
+    if (a.M < ((int64_t)1 << 31)) return a.L >= a.M ? 0 : (int64_t)((uint32_t)row / (uint32_t)a.L);
+    return row / a.L;
+}
 // whether the row is sampled at all; otherwise its token stays
 __device__ __forceinline__ bool row_moves(const SampleArgs& a, int64_t row, int64_t b) {
     if (!a.xcur) return true;
@@ -64,12 +71,11 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 // u + 1e-10 in 32 bits as the reference's catsample rounds it, kept inside (0, 1] whatever u is
 __device__ __forceinline__ float noise_arg(float u) { return __builtin_amdgcn_fmed3f(u + 1e-10f, 1e-10f, 1.0f); }
 
-// ------------------------------------------------------------------------------- the definition itself, in 64 bits
-// NT threads (a power of two of whole waves) work one row together, reading it from memory in every pass.
+// NT threads (a power of two of whole waves) joined over one row in 64 bits
 template <int NT> struct Joint {
     double* sd;  // [NT / 64] each
     int64_t* si;
-    template <typename F> __device__ __forceinline__ double dsum(double v, F) {
+    __device__ __forceinline__ double sum(double v) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
         if constexpr (NT == 64) return v;
@@ -80,7 +86,6 @@ template <int NT> struct Joint {
         for (int w = 1; w < NT / 64; ++w) v += sd[w];
         return v;
     }
-    __device__ __forceinline__ double sum(double v) { return dsum(v, 0); }
     __device__ __forceinline__ int64_t isum(int64_t v) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -111,102 +116,18 @@ template <int NT> struct Joint {
     }
 };
 
-template <typename T, int NT>
-__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, double* sd, int64_t* si) {
-    Joint<NT> J{sd, si};
-    const int lane = threadIdx.x & (NT - 1), V = a.V;
-    const T* x = (const T*)a.x + row * a.ld;
-    const float* u = a.u + row * a.ldu;
-    const RowParams rp = row_params(a, b);
-    const int64_t none = (int64_t)1 << 40;
-    // the first entry of the order
-    double mxd = -1.0;  // (as an order key, so that one reduction serves)
-    int64_t mi = none;
-    for (int j = lane; j < V; j += NT) {
-        const uint32_t key = order_key(to_f32<T>(x[j]));
-        if (key && (double)key > mxd) { mxd = (double)key; mi = j; }
-    }
-    J.best(mxd, mi);
-    if (mi == none) return row_empty(a);
-    if (!(rp.T > 0.f)) return mi;  // greedy
-    const uint32_t kmax = (uint32_t)mxd;
-    const double mx = (double)(to_f32<T>(x[mi]) + 0.0f), rT = (double)rp.T;
-    const bool top_inf = isinf(mx);
-    auto weight = [&](uint32_t key, float v) -> double {
-        if (key == kmax) return 1.0;
-        return top_inf ? 0.0 : exp(((double)v - mx) / rT);
-    };
-    // mass of the k first of the order
-    double W = 0.0;
-    if (rp.P < 1.f) {
-        uint32_t t = 0;  // the k-th largest key, or 0 if there are no k candidates
-        if (rp.k < V) {
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t c = t | (1u << bit);
-                int64_t n = 0;
-                for (int j = lane; j < V; j += NT) n += order_key(to_f32<T>(x[j])) >= c;
-                if (J.isum(n) >= rp.k) t = c;
-            }
-        }
-        double s = 0.0, q = 0.0;
-        int64_t n = 0;
-        for (int j = lane; j < V; j += NT) {
-            const float v = to_f32<T>(x[j]);
-            const uint32_t key = order_key(v);
-            if (key > t) { s += weight(key, v); ++n; }
-            else if (key == t && t) q = weight(key, v);
-        }
-        W = J.sum(s);
-        if (t) {
-            n = J.isum(n);
-            int64_t dummy = 0;
-            J.best(q, dummy);
-            W += (double)(rp.k - n) * q;  // of equal entries at the border the lowest indices are in; they weigh the same
-        }
-    }
-    uint32_t kc = 0xffffffffu;  // what is still possible: ranked before (kc, ic)
-    int64_t ic = none;
-    for (;;) {
-        double bv = -1.0;
-        int64_t bi = none;
-        for (int j = lane; j < V; j += NT) {
-            const float v = to_f32<T>(x[j]);
-            const uint32_t key = order_key(v);
-            if (!key || !(key > kc || (key == kc && j < ic) || ic == none)) continue;
-            const double r = weight(key, v) / (1e-10 - log((double)noise_arg(u[j])));
-            if (r > bv) { bv = r; bi = j; }
-        }
-        J.best(bv, bi);
-        if (bi == none) return mi;  // (cannot be: the first of the order is always kept)
-        const float vw = to_f32<T>(x[bi]);
-        const uint32_t kw = order_key(vw);
-        double S = 0.0;
-        int64_t rank = 0;
-        for (int j = lane; j < V; j += NT) {
-            const float v = to_f32<T>(x[j]);
-            const uint32_t key = order_key(v);
-            if (key > kw || (key == kw && j < bi)) { S += weight(key, v); ++rank; }
-        }
-        rank = J.isum(rank);
-        if (rank == 0) return bi;
-        S = J.sum(S);
-        if (rank < rp.k && (!(rp.P < 1.f) || S < (double)rp.P * W) && !(weight(kw, vw) < (double)rp.m)) return bi;
-        kc = kw;
-        ic = bi;
-    }
-}
-
 // ------------------------------------------------------------------------------------------- the same in 32 bits
 // Per row the 32-bit pass either settles the decision or gives the row up to resolve_row64.  What its quantities are off by
 // (v_exp_f32, v_log_f32 and v_rcp_f32 measured below 2^-23 relative):
 //   q_j: d2 = (x - max) * (log2 e / T) has four roundings, so q_j is off by |d2| 4 2^-24 ln 2 + 2^-23 relative.
 //   q_j / E_j: a winner has q_j >= (1 / 23.1) * 1e-10, the smallest E over the largest (the first of the order has q = 1), so
-//     |d2| <= 39 and the ratio is off by 7.2e-6; two of them are told apart when they differ by more than 1.45e-5: RATIO_TOL.
+//     |d2| <= 38 and the ratio is off by 7.0e-6; two of them are told apart when they differ by more than 1.4e-5: RATIO_TOL.
 //   S, W: sum q |d2| <= W log2 V, so a sum is off by (log2 V * 2.8 + 2) 2^-24 W and by its n adds one after the other, n 2^-24 W:
 //     V <= 64 in one lane 5.0e-6 W; 64 a lane and 10 across, V = 32768: 7.1e-6 W.  S against P W: 1.42e-5 W at most: MASS_TOL.
-// A comparison nearer than that, and every row whose maximum or temperature leaves the range of these bounds, is "near".
-#define RATIO_TOL 0x1p-15f
-#define MASS_TOL 0x1p-15f
+// Both tolerances are 1.53e-5.  A comparison nearer than that, and every row whose maximum or temperature leaves the range of
+// these bounds, is "near": about one row in 30000 with top-p.
+#define RATIO_TOL 0x1p-16f
+#define MASS_TOL 0x1p-16f
 #define LOG2E 1.44269504f
 #define LN2 0.693147181f
 
@@ -238,6 +159,135 @@ __device__ __forceinline__ Verdict judge(const RowParams& rp, int rank, float S,
     return second < best * (1.f - RATIO_TOL) ? KEPT : NEAR;
 }
 
+// ------------------------------------------------------------------------------- the definition itself, in 64 bits
+// Reads the row again in every pass: for rows that came near, for rows outside the range of the 32-bit bounds, and for rows too
+// long for registers; xs: LDS for the scores of a row, if it fits.  Within that range the arg-max is looked for among the entries whose 32-bit ratio comes within twice the
+// tolerance of the largest, usually one or two, and only those are evaluated in 64 bits.
+template <typename T, int NT>
+__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, double* sd, int64_t* si, float* xs = nullptr) {
+    Joint<NT> J{sd, si};
+    const int lane = threadIdx.x & (NT - 1), V = a.V;
+    const T* px = (const T*)a.x + row * a.ld;
+    const float* u = a.u + row * a.ldu;
+    if (xs) {
+        __syncthreads();
+#pragma unroll 4
+        for (int j = lane; j < V; j += NT) xs[j] = to_f32<T>(px[j]);
+        __syncthreads();
+    }
+    auto score = [&](int64_t j) { return xs ? xs[j] : to_f32<T>(px[j]); };
+    const RowParams rp = row_params(a, b);
+    const int64_t none = (int64_t)1 << 40;
+    // the first entry of the order
+    double mxd = -1.0;  // (as an order key, so that one reduction serves)
+    int64_t mi = none;
+#pragma unroll 4
+    for (int j = lane; j < V; j += NT) {
+        const uint32_t key = order_key(score(j));
+        if (key && (double)key > mxd) { mxd = (double)key; mi = j; }
+    }
+    J.best(mxd, mi);
+    if (mi == none) return row_empty(a);
+    if (!(rp.T > 0.f)) return mi;  // greedy
+    const uint32_t kmax = (uint32_t)mxd;
+    const float mxf = score(mi) + 0.0f;
+    const double mx = (double)mxf, rT = (double)rp.T;
+    const bool top_inf = isinf(mx);
+    auto weight = [&](uint32_t key, float v) -> double {
+        if (key == kmax) return 1.0;
+        return top_inf ? 0.0 : exp(((double)v - mx) / rT);
+    };
+    auto ratio = [&](uint32_t key, float v, int64_t j) { return weight(key, v) / (1e-10 - log((double)noise_arg(u[j]))); };
+    bool beyond = top_inf;
+    const float c = rate_of(rp.T, beyond);
+    const bool fast = !beyond;
+    // mass of the k first of the order (when it is needed)
+    double W = -1.0;
+    auto mass = [&]() {
+        uint32_t t = 0;
+        if (rp.k < V) {  // the k-th largest key; 0 if there are no k candidates
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t ct = t | (1u << bit);
+                int64_t n = 0;
+#pragma unroll 4
+                for (int j = lane; j < V; j += NT) n += order_key(score(j)) >= ct;
+                n = J.isum(n);
+                if (n >= rp.k) t = ct;
+                if (n == rp.k) break;  // (then exactly the k first are at or above t)
+            }
+        }
+        double s = 0.0, q = 0.0;
+        int64_t n = 0;
+#pragma unroll 4
+        for (int j = lane; j < V; j += NT) {
+            const float v = score(j);
+            const uint32_t key = order_key(v);
+            if (key > t) { s += weight(key, v); ++n; }
+            else if (key == t && t) q = weight(key, v);
+        }
+        W = J.sum(s);
+        if (t) {
+            n = J.isum(n);
+            int64_t dummy = 0;
+            J.best(q, dummy);
+            W += (double)(rp.k - n) * q;  // of equal entries at the border the lowest indices are in; they weigh the same
+        }
+    };
+    uint32_t kc = 0xffffffffu;  // what is still possible: ranked before (kc, ic)
+    int64_t ic = none;
+    for (;;) {
+        double bv = -1.0, least = -1.0;
+        int64_t bi = none;
+        auto possible = [&](uint32_t key, int64_t j) { return key && (key > kc || (key == kc && j < ic) || ic == none); };
+        auto ratio32 = [&](float v, int64_t j) { return (double)(__builtin_amdgcn_exp2f((v - mxf) * c) * inv_noise(u[j])); };
+        if (fast) {
+            int64_t any = 0;
+#pragma unroll 4
+            for (int j = lane; j < V; j += NT) {
+                const float v = score(j);
+                const double r = ratio32(v, j);
+                if (possible(order_key(v), j) && r > least) least = r;
+            }
+            J.best(least, any);
+            least *= 1.0 - 2.0 * RATIO_TOL;
+        }
+#pragma unroll 4
+        for (int j = lane; j < V; j += NT) {
+            const float v = score(j);
+            const uint32_t key = order_key(v);
+            if (!possible(key, j) || (fast && ratio32(v, j) < least)) continue;
+            const double r = ratio(key, v, j);
+            if (r > bv) { bv = r; bi = j; }
+        }
+        J.best(bv, bi);
+        if (bi == none) return mi;  // (cannot be: the first of the order is always kept)
+        const float vw = score(bi);
+        const uint32_t kw = order_key(vw);
+        int64_t rank = 0;
+#pragma unroll 4
+        for (int j = lane; j < V; j += NT) {
+            const uint32_t key = order_key(score(j));
+            rank += (key > kw) | ((key == kw) & (j < bi));
+        }
+        rank = J.isum(rank);
+        if (rank == 0) return bi;
+        if (rank < rp.k && !(weight(kw, vw) < (double)rp.m)) {
+            if (!(rp.P < 1.f)) return bi;
+            if (W < 0.0) mass();
+            double S = 0.0;
+#pragma unroll 4
+            for (int j = lane; j < V; j += NT) {
+                const float v = score(j);
+                const uint32_t key = order_key(v);
+                if (key > kw || (key == kw && j < bi)) S += weight(key, v);
+            }
+            if (J.sum(S) < (double)rp.P * W) return bi;
+        }
+        kc = kw;
+        ic = bi;
+    }
+}
+
 // ---- V <= 64: a lane owns a row.  Everything is register arithmetic over the lane's own entries, no cross-lane traffic; the
 // rows of a wave are neighbours in memory, so the loads of a wave cover one stretch of it.  In the middle of a sampler run most
 // rows are not sampled: a block packs those that are to its first lanes, and the waves behind them end.
@@ -262,12 +312,16 @@ template <typename T, int VP>
 __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
     __shared__ int s_cnt;
     __shared__ uint8_t s_list[256];
-    const int64_t row0 = (int64_t)blockIdx.x * 256, b0 = row0 / a.L, off0 = row0 - b0 * a.L;
+    const int64_t row0 = (int64_t)blockIdx.x * 256;
+    const bool per = a.T || a.P || a.m || a.k || a.move;
+    const int64_t b0 = per ? (a.M < ((int64_t)1 << 31) ? (int64_t)((uint32_t)row0 / (uint32_t)(a.L < a.M ? a.L : a.M)) : row0 / a.L) : 0;
+    const int64_t off0 = row0 - b0 * a.L;
     const int V = a.V, lane = threadIdx.x & 63;
     int r = threadIdx.x;
     bool on = row0 + r < a.M;
     auto batch_of = [&](int rr) -> int64_t {
         const int64_t q = off0 + rr;
+        if (!per) return 0;
         return a.L >= 256 ? b0 + (q >= a.L) : b0 + (uint32_t)q / (uint32_t)a.L;
     };
     if (a.xcur) {  // (uniform: the barriers are met by the whole block)
@@ -414,7 +468,7 @@ struct Best {
 // one lane's numbers joined over the NW waves of a row; every member is called by all of them.  The exchange alternates
 // between two buffers, so a barrier per call is enough: a buffer is written again two calls later.
 template <int NW> struct RowRed {
-    float (*buf)[6 * NW];
+    float (*buf)[4 * NW];
     int turn = 0;
     __device__ __forceinline__ float max(float v) {
         v = dpp_max(v);
@@ -445,23 +499,30 @@ template <int NW> struct RowRed {
         }
         return n;
     }
-    // joins `v`, and the sum and the count beside it
-    __device__ __forceinline__ void join(Best& v, float& s, int& n) {
+    // the best of all lanes
+    __device__ __forceinline__ void best(Best& v) {
         pick(v, 64);
+        if constexpr (NW > 1) {
+            float* o = swap();
+            const int w = threadIdx.x >> 6, l = threadIdx.x & (NW - 1);
+            if ((threadIdx.x & 63) == 0) { o[w] = v.b1; o[NW + w] = v.b2; o[2 * NW + w] = v.x; o[3 * NW + w] = __int_as_float(v.i); }
+            __syncthreads();
+            v = {o[l], o[NW + l], o[2 * NW + l], __float_as_int(o[3 * NW + l])};
+            pick(v, NW);
+        }
+    }
+    // a sum over lanes and two counts of the wave
+    __device__ __forceinline__ void sums(float& s, int& n, int& m) {
         s = dpp_sum(s);
         if constexpr (NW > 1) {
             float* o = swap();
             const int w = threadIdx.x >> 6, l = threadIdx.x & (NW - 1);
-            if ((threadIdx.x & 63) == 0) {
-                o[w] = v.b1; o[NW + w] = v.b2; o[2 * NW + w] = v.x; o[3 * NW + w] = __int_as_float(v.i);
-                o[4 * NW + w] = s; o[5 * NW + w] = (float)n;
-            }
+            if ((threadIdx.x & 63) == 0) { o[w] = s; o[NW + w] = (float)n; o[2 * NW + w] = (float)m; }
             __syncthreads();
-            v = {o[l], o[NW + l], o[2 * NW + l], __float_as_int(o[3 * NW + l])};
             const bool mine = (threadIdx.x & 63) < NW;
-            s = dpp_sum(mine ? o[4 * NW + l] : 0.f);
-            n = (int)dpp_sum(mine ? o[5 * NW + l] : 0.f);
-            pick(v, NW);
+            s = dpp_sum(mine ? o[l] : 0.f);
+            n = (int)dpp_sum(mine ? o[NW + l] : 0.f);
+            m = (int)dpp_sum(mine ? o[2 * NW + l] : 0.f);
         }
     }
 
@@ -501,11 +562,12 @@ template <int LOW, int N, class R> __device__ __forceinline__ uint32_t kth_key(c
 template <int N, class R>
 __device__ __forceinline__ float mass_of_first(const float (&x)[N], int k, uint32_t t, float mx, float c, R& red) {
     const float tv = key_value(t);
-    float s = 0.f;
+    float s = 0.f, mm = mx;
     int n = 0;
+    asm volatile("" : "+v"(mm));  // (not kept from the first pass, as in eliminate)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        s += x[i] > tv ? __builtin_amdgcn_exp2f((x[i] - mx) * c) : 0.f;
+        s += x[i] > tv ? __builtin_amdgcn_exp2f((x[i] - mm) * c) : 0.f;
         n += __popcll(__ballot(x[i] > tv));
     }
     s = red.sum(s);
@@ -517,83 +579,115 @@ __device__ __forceinline__ float mass_of_first(const float (&x)[N], int k, uint3
     at = red.max(at);
     return at > -INFINITY ? s + (float)(k - n) * __builtin_amdgcn_exp2f((tv - mx) * c) : s;
 }
-// the elimination over entries (x[i], index jof(i)) with ratios r[i] (-1: no candidate)
+// the best of the entries before (xw, index off + jw) — of all, if there is no such entry yet (xw = +inf)
 template <int N, class R, class J>
-__device__ __forceinline__ int eliminate(const RowParams& rp, bool cut, const float (&x)[N], const float (&r)[N], J jof,
-                                         float mx, float c, float W, R& red, bool& near) {
+__device__ __forceinline__ Best best_before(const float (&x)[N], const float (&r)[N], J jc, int off, float xw, int jw, bool tied, R& red) {
     Best v{-1.f, -1.f, 0.f, 0};
+    if (tied) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        v.b2 = __builtin_amdgcn_fmed3f(v.b1, v.b2, r[i]);
-        v.i = r[i] > v.b1 ? i : v.i;
-        v.x = r[i] > v.b1 ? x[i] : v.x;
-        v.b1 = fmaxf(v.b1, r[i]);
+        for (int i = 0; i < N; ++i) {
+            const float ri = (x[i] > xw) | ((x[i] == xw) & (jc(i) < jw)) ? r[i] : -1.f;
+            v.b2 = __builtin_amdgcn_fmed3f(v.b1, v.b2, ri);
+            v.i = ri > v.b1 ? i : v.i;
+            v.x = ri > v.b1 ? x[i] : v.x;
+            v.b1 = fmaxf(v.b1, ri);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float ri = x[i] > xw ? r[i] : -1.f;
+            v.b2 = __builtin_amdgcn_fmed3f(v.b1, v.b2, ri);
+            v.i = ri > v.b1 ? i : v.i;
+            v.x = ri > v.b1 ? x[i] : v.x;
+            v.b1 = fmaxf(v.b1, ri);
+        }
     }
-    v.i = jof(v.i);
-    float s = 0.f;
-    int rank = 0;
-    red.join(v, s, rank);
+    v.i = off + jc(v.i);
+    red.best(v);
+    return v;
+}
+// the elimination over entries (x[i], index off + jc(i)) with ratios r[i] (-1: no candidate).  What a pass can compute again
+// (the weights, the indexes) it does: kept from pass to pass it would take as many registers as the row.  Equal scores are
+// rare, so the order among them costs a pass of its own when the candidate is not alone at its score.
+template <bool RANK, int N, class R, class J>
+__device__ __forceinline__ int eliminate(const RowParams& rp, bool cut, const float (&x)[N], const float (&r)[N], J jc, int off,
+                                         float mx, float c, float W, R& red, bool& near) {
+    Best v = best_before(x, r, jc, off, -INFINITY, 0, false, red);
     if (!cut) {
         near = !(v.b2 < v.b1 * (1.f - RATIO_TOL));
         return v.i;
     }
     for (;;) {
-        Best w{-1.f, -1.f, 0.f, 0};
-        s = 0.f;
-        rank = 0;
+        float cc = c, mm = mx, s = 0.f;
+        asm volatile("" : "+v"(cc), "+v"(mm));
+        int above = 0, equal = 0, ties = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const bool before = (x[i] > v.x) | ((x[i] == v.x) & (jof(i) < v.i));
-            const float q = __builtin_amdgcn_exp2f((x[i] - mx) * c), ri = before ? r[i] : -1.f;
-            s += before ? q : 0.f;
-            rank += __popcll(__ballot(before));
-            w.b2 = __builtin_amdgcn_fmed3f(w.b1, w.b2, ri);
-            w.i = ri > w.b1 ? i : w.i;
-            w.x = ri > w.b1 ? x[i] : w.x;
-            w.b1 = fmaxf(w.b1, ri);
+            const bool gt = x[i] > v.x;
+            s += gt ? __builtin_amdgcn_exp2f((x[i] - mm) * cc) : 0.f;
+            if constexpr (RANK) above += __popcll(__ballot(gt));
+            equal += __popcll(__ballot(x[i] == v.x));
         }
-        w.i = jof(w.i);
-        red.join(w, s, rank);
-        const Verdict d = judge(rp, rank, s, W, __builtin_amdgcn_exp2f((v.x - mx) * c), v.b1, v.b2);
+        red.sums(s, above, equal);
+        const float q = __builtin_amdgcn_exp2f((v.x - mm) * cc);
+        if (equal > 1) {
+            const int vi = v.i - off;
+#pragma unroll
+            for (int i = 0; i < N; ++i) ties += __popcll(__ballot((x[i] == v.x) & (jc(i) < vi)));
+            ties = red.count(ties);
+            s += (float)ties * q;
+        }
+        const int rank = RANK ? above + ties : (v.x == mx ? ties : ties + 1);  // (without RANK only whether it is 0 matters)
+        const Verdict d = judge(rp, rank, s, W, q, v.b1, v.b2);
         if (d != DROPPED) {
             near = d == NEAR;
             return v.i;
         }
-        v = w;
+        v = best_before(x, r, jc, off, v.x, v.i - off, equal > 1, red);
     }
 }
 
 // Where top-k or min-p leaves few entries, they are packed, four to a lane of one wave, and only their noise is read:
 // the k-th largest of the lanes' own maxima is a bound that at least k entries reach (k distinct lanes), usually not many more.
 #define PACK 256
+template <int NW> struct WideShared {
+    static constexpr int ROWS = NW == 1 ? 4 : 1;
+    float x[ROWS][PACK];
+    int j[ROWS][PACK];
+    float red[2][4 * NW];
+    int n, ans;
+};
+// the token of a row that is sampled; near: it is not settled
 template <typename T, int NW, int NE>
-__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64) sample_wide_kernel(SampleArgs a) {
-    constexpr int NT = NW * 64, ROWS = NW == 1 ? 4 : 1, LOW = sizeof(T) == 2 ? 16 : 0;
-    __shared__ float s_x[ROWS][PACK];
-    __shared__ int s_j[ROWS][PACK];
-    __shared__ float s_red[2][6 * NW];
-    __shared__ double s_d[NW];
-    __shared__ int64_t s_i[NW];
-    __shared__ int s_n, s_ans, s_near;
+__device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, int64_t b, WideShared<NW>& sh, bool& near) {
+    constexpr int NT = NW * 64, LOW = sizeof(T) == 2 ? 16 : 0;
     const int V = a.V, lane = threadIdx.x & 63, tid = NW == 1 ? lane : (int)threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = NW == 1 ? wave : 0;
-    RowRed<NW> red{s_red};
+    RowRed<NW> red{sh.red};
     RowRed<1> alone{nullptr};
     auto jof = [&](int i) { return (i >> 2) * (4 * NT) + tid * 4 + (i & 3); };
-    // (One row per wave and launch, no loop: out of one, the constants of the 64-bit exp and log would be hoisted and kept in
-    // a hundred registers.)
-    const int64_t row = (int64_t)blockIdx.x * ROWS + slot;
     {
-        if (row >= a.M) return;
-        const int64_t b = row / a.L;
-        if (!row_moves(a, row, b)) {
-            if (tid == 0) a.out[row] = a.xcur[row];
-            return;
-        }
         RowParams rp = row_params(a, b);
         const T* px = (const T*)a.x + row * a.ld;
         const float* pu = a.u + row * a.ldu;
-        float x[NE], top = -INFINITY;
+        float x[NE], r[NE], top = -INFINITY;
+        // the noise: at once where no truncation can pack the row, else when it is known what of it is read
+        auto read_noise = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < NE; i += 4) {
+                const int j = jof(i);
+                if (j + 4 <= V) {
+                    struct __attribute__((packed)) { float e[4]; } v;
+                    __builtin_memcpy(&v, pu + j, 16);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) r[i + k] = v.e[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) r[i + k] = j + k < V ? pu[j + k] : 0.5f;
+                }
+            }
+        };
+        const bool whole = rp.k >= V && (rp.P < 1.f || !(rp.m > 0.f)) && rp.T > 0.f;
 #pragma unroll
         for (int i = 0; i < NE; i += 4) {
             const int j = jof(i);
@@ -607,17 +701,15 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64) sample_wide_kernel(Sa
                 for (int k = 0; k < 4; ++k) x[i + k] = j + k < V ? to_f32<T>(px[j + k]) : -INFINITY;
             }
         }
+        if (whole) read_noise();
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
             x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;
             top = fmaxf(top, x[i]);
         }
         const float mx = red.max(top);
-        if (!(mx > -INFINITY)) {
-            if (tid == 0) a.out[row] = row_empty(a);
-            return;
-        }
-        bool near = mx == INFINITY;
+        if (!(mx > -INFINITY)) return row_empty(a);
+        near = mx == INFINITY;
         int got = -1;
         if (!(rp.T > 0.f)) {
             float first = -INFINITY;  // (an index is below 2^24)
@@ -661,10 +753,10 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64) sample_wide_kernel(Sa
                 if (n <= PACK && (rp.k < V || !(rp.P < 1.f))) {
                     int base = 0;
                     if constexpr (NW > 1) {
-                        if (threadIdx.x == 0) s_n = 0;
+                        if (threadIdx.x == 0) sh.n = 0;
                         __syncthreads();
                         const int mine = reach();
-                        if (lane == 0) base = atomicAdd(&s_n, mine);  // (the order of the packed entries does not matter)
+                        if (lane == 0) base = atomicAdd(&sh.n, mine);  // (the order of the packed entries does not matter)
                         base = __builtin_amdgcn_readfirstlane(base);
                     }
 #pragma unroll
@@ -673,74 +765,94 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64) sample_wide_kernel(Sa
                         const unsigned long long mask = __ballot(in);
                         if (in) {
                             const int at = base + __popcll(mask & ((1ull << lane) - 1ull));
-                            s_x[slot][at] = x[i];
-                            s_j[slot][at] = jof(i);
+                            sh.x[slot][at] = x[i];
+                            sh.j[slot][at] = jof(i);
                         }
                         base += __popcll(mask);
                     }
                     if constexpr (NW > 1) __syncthreads();
                     else __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order)
                     if (NW == 1 || wave == 0) {
-                        float y[4], r[4];
+                        float y[4], ry[4];
                         int jj[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int e = lane + 64 * i;
-                            y[i] = e < n ? s_x[slot][e] : -INFINITY;
-                            jj[i] = e < n ? s_j[slot][e] : 0;
-                            r[i] = e < n ? __builtin_amdgcn_exp2f((y[i] - mx) * c) * inv_noise(pu[jj[i]]) : -1.f;
+                            y[i] = e < n ? sh.x[slot][e] : -INFINITY;
+                            jj[i] = e < n ? sh.j[slot][e] : 0;
+                            ry[i] = e < n ? __builtin_amdgcn_exp2f((y[i] - mx) * c) * inv_noise(pu[jj[i]]) : -1.f;
                         }
                         float W = 0.f;
                         if (rp.P < 1.f) {
                             if (!t) t = kth_key<LOW>(y, rp.k, alone);
                             W = mass_of_first(y, rp.k, t, mx, c, alone);
                         }
-                        got = eliminate<4>(rp, cut, y, r, [&](int i) { return i == 0 ? jj[0] : i == 1 ? jj[1] : i == 2 ? jj[2] : jj[3]; },
-                                           mx, c, W, alone, near);
+                        got = eliminate<true, 4>(rp, cut, y, ry, [&](int i) { return i == 0 ? jj[0] : i == 1 ? jj[1] : i == 2 ? jj[2] : jj[3]; }, 0,
+                                                 mx, c, W, alone, near);
                         if constexpr (NW > 1) {
-                            if (lane == 0) { s_ans = got; s_near = near; }
+                            if (lane == 0) sh.ans = near ? -1 : got;
                         }
                     }
                     if constexpr (NW > 1) {
                         __syncthreads();
-                        got = s_ans;
-                        near = s_near != 0;
+                        got = sh.ans;
+                        near = got < 0;
                     } else {
                         __builtin_amdgcn_wave_barrier();
                     }
                 } else {
-                    float r[NE], W = 0.f;
+                    float W = 0.f;
+                    if (!whole) read_noise();
 #pragma unroll
-                    for (int i = 0; i < NE; i += 4) {
-                        const int j = jof(i);
-                        float u4[4];
-                        if (j + 4 <= V) {
-                            struct __attribute__((packed)) { float e[4]; } v;
-                            __builtin_memcpy(&v, pu + j, 16);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) u4[k] = v.e[k];
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) u4[k] = j + k < V ? pu[j + k] : 0.5f;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float q = __builtin_amdgcn_exp2f((x[i + k] - mx) * c);
-                            W += q;
-                            r[i + k] = ((x[i + k] >= thr) & (x[i + k] > -INFINITY)) ? q * inv_noise(u4[k]) : -1.f;
-                        }
+                    for (int i = 0; i < NE; ++i) {
+                        const float q = __builtin_amdgcn_exp2f((x[i] - mx) * c);
+                        W += q;
+                        r[i] = ((x[i] >= thr) & (x[i] > -INFINITY)) ? q * inv_noise(r[i]) : -1.f;
                     }
                     if (rp.P < 1.f) W = t ? mass_of_first(x, rp.k, t, mx, c, red) : red.sum(W);
-                    got = eliminate<NE>(rp, cut, x, r, jof, mx, c, W, red, near);
+                    auto jc = [&](int i) { return (i >> 2) * (4 * NT) + (i & 3); };
+                    if (rp.k < V) got = eliminate<true, NE>(rp, cut, x, r, jc, tid * 4, mx, c, W, red, near);
+                    else got = eliminate<false, NE>(rp, cut, x, r, jc, tid * 4, mx, c, W, red, near);
                 }
             }
         }
-        int64_t ans = got;
-        if (near) {
-            if constexpr (NW > 1) __syncthreads();
-            ans = resolve_row64<T, NT>(a, row, b, s_d, s_i);
+        return got;
+    }
+}
+
+// A row that came near gets this in place of its token until sample_near_kernel, launched behind, has decided it: kept in this
+// kernel, the 64-bit arithmetic would take its registers (115 instead of 60) and half of its waves (131072 x 300: 159 us with it,
+// 79 us and 4 us for the launch behind without), and one wave alone with a row would be the last of the launch by 50 us.
+#define NEAR_TOKEN INT64_MIN
+#define NEAR_ROW 12288
+template <typename T, int NW, int NE>
+__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sample_wide_kernel(SampleArgs a) {
+    __shared__ WideShared<NW> sh;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+    if (row >= a.M) return;
+    const int64_t b = batch_of_row(a, row);
+    bool near = false;
+    const int64_t ans = row_moves(a, row, b) ? wide_row<T, NW, NE>(a, row, b, sh, near) : a.xcur[row];
+    if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN : ans;
+}
+// a block looks through `per` rows (at most 256) and takes those that came near one after the other
+template <typename T> __global__ void __launch_bounds__(256) sample_near_kernel(SampleArgs a, int per) {
+    __shared__ double sd[4];
+    __shared__ int64_t si[4];
+    __shared__ uint64_t s_mask[4];
+    __shared__ float s_row[NEAR_ROW];
+    const int64_t row0 = (int64_t)blockIdx.x * per, mine = row0 + threadIdx.x;
+    const bool near = (int)threadIdx.x < per && mine < a.M && a.out[mine] == NEAR_TOKEN;
+    const uint64_t mask = __ballot(near);
+    if ((threadIdx.x & 63) == 0) s_mask[threadIdx.x >> 6] = mask;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+        for (uint64_t todo = s_mask[w]; todo; todo &= todo - 1) {
+            const int64_t row = row0 + w * 64 + __builtin_ctzll(todo);
+            const int64_t ans = resolve_row64<T, 256>(a, row, batch_of_row(a, row), sd, si, a.V <= NEAR_ROW ? s_row : nullptr);
+            if (threadIdx.x == 0) a.out[row] = ans;
         }
-        if (tid == 0) a.out[row] = ans;
     }
 }
 
@@ -749,7 +861,7 @@ __global__ void __launch_bounds__(NT) sample_row64_kernel(SampleArgs a) {
     __shared__ double sd[NT / 64];
     __shared__ int64_t si[NT / 64];
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        const int64_t b = row / a.L;
+        const int64_t b = batch_of_row(a, row);
         int64_t got;
         if (!row_moves(a, row, b)) got = a.xcur[row];
         else got = resolve_row64<T, NT>(a, row, b, sd, si);
@@ -763,6 +875,9 @@ template <typename T, int VP> static void launch_lane(const SampleArgs& a, hipSt
 template <typename T, int NW, int NE> static void launch_wide(const SampleArgs& a, hipStream_t st) {
     constexpr int R = NW == 1 ? 4 : 1;
     hipLaunchKernelGGL((sample_wide_kernel<T, NW, NE>), dim3((unsigned)((a.M + R - 1) / R)), dim3(NW == 1 ? 256 : NW * 64), 0, st, a);
+    int64_t per = (a.M + 2047) / 2048;
+    per = per > 256 ? 256 : per;
+    hipLaunchKernelGGL((sample_near_kernel<T>), dim3((unsigned)((a.M + per - 1) / per)), dim3(256), 0, st, a, (int)per);
 }
 template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t st) {
     // V up to a multiple of 4 (8 above 32): the entries behind V cost arithmetic, and a row is never read past its end
@@ -783,6 +898,7 @@ template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t
     else if (a.V <= 512) launch_wide<T, 1, 8>(a, st);
     else if (a.V <= 1024) launch_wide<T, 1, 16>(a, st);
     else if (a.V <= 2048) launch_wide<T, 1, 32>(a, st);
+    else if (a.V <= 2560) launch_wide<T, 1, 40>(a, st);
     else if (a.V <= 48 * 64) launch_wide<T, 1, 48>(a, st);
     else if (a.V <= 4096) launch_wide<T, 1, 64>(a, st);
     else if (a.V <= 8192) launch_wide<T, 4, 32>(a, st);
