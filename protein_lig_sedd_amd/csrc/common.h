@@ -62,6 +62,31 @@ template <int G> __device__ __forceinline__ void group_argmax(float& v, int& idx
 }
 __device__ __forceinline__ float wave_sum(float v) { return group_sum<64>(v); }
 
+// ---- sums and maxima over a whole wave by DPP moves (four steps inside rows of 16 lanes, two across them, then lane 63's value to
+// all): arithmetic latency only, where a shuffle goes through the LDS crossbar at every step.  All 64 lanes must be active.
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_f(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ float dpp_sum(float v) {
+    v += dpp_f<0x111, 0xf>(0.f, v);
+    v += dpp_f<0x112, 0xf>(0.f, v);
+    v += dpp_f<0x114, 0xf>(0.f, v);
+    v += dpp_f<0x118, 0xf>(0.f, v);
+    v += dpp_f<0x142, 0xa>(0.f, v);
+    v += dpp_f<0x143, 0xc>(0.f, v);
+    return lane63(v);
+}
+__device__ __forceinline__ float dpp_max(float v) {
+    v = fmaxf(v, dpp_f<0x111, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x112, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x114, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x118, 0xf>(v, v));
+    v = fmaxf(v, dpp_f<0x142, 0xa>(v, v));
+    v = fmaxf(v, dpp_f<0x143, 0xc>(v, v));
+    return lane63(v);
+}
+
 // e^sigma - 1 as the reference computes it (graph_lib.py:279-283)
 __device__ __forceinline__ float esigm1f(float s) { return s < 0.5f ? expm1f(s) : expf(s) - 1.0f; }
 

@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(TPB) post_norm_fwd_kernel(
         }
         s += (v[k].x + v[k].y) + (v[k].z + v[k].w);
     }
-    const float pm = wave_sum(s) * inv_d;
+    const float pm = dpp_sum(s) * inv_d;
     float q = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(TPB) post_norm_fwd_kernel(
             q += (v[k].x * v[k].x + v[k].y * v[k].y) + (v[k].z * v[k].z + v[k].w * v[k].w);
         }
     }
-    const float pr = 1.0f / sqrtf(wave_sum(q) * inv_d + 1e-5f);
+    const float pr = 1.0f / sqrtf(dpp_sum(q) * inv_d + 1e-5f);
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(TPB) post_norm_fwd_kernel(
     }
     if (lane == 0) { pmean[row] = pm; prstd[row] = pr; }
     if constexpr (NEXT) {
-        const float mu = wave_sum(s) * inv_d;
+        const float mu = dpp_sum(s) * inv_d;
         q = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(TPB) post_norm_fwd_kernel(
                 q += (v[k].x * v[k].x + v[k].y * v[k].y) + (v[k].z * v[k].z + v[k].w * v[k].w);
             }
         }
-        const float r1 = 1.0f / sqrtf(wave_sum(q) * inv_d + 1e-5f);
+        const float r1 = 1.0f / sqrtf(dpp_sum(q) * inv_d + 1e-5f);
         if (lane == 0) { mean[row] = mu; rstd[row] = r1; }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -150,29 +150,35 @@ extern "C" int sedd_post_norm_residual_fwd(const float* residual, const void* a,
 // da  = pr * (g2 - mean(g2) - ahat * mean(g2 ahat)),     g2 = dn * wp
 // dw += dh (1 + scale) xhat;  dshift = sum dh;  dscale = sum dh xhat w;  dgate = sum d keep ahat wp;  dwp += dn ahat;
 // dbias += da (before it is rounded: the bias gradient of the Linear that made a)
-// A block owns a chunk of at most 32 / 64 rows of one batch element and a thread four columns of it, so the six column
-// sums are running sums in registers and leave as one line of partial sums per chunk: no fold across waves, which a
-// wave-per-row layout needs for all six.  What crosses the waves is two pairs of row sums, through LDS, for POST_ROWS rows
-// at a time.
-#ifndef POST_ROWS
-#define POST_ROWS 2
-#endif
-template <int N> __device__ __forceinline__ void block_sums(float (&v)[N], float* buf, int nw) {
-    const int wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+// A block owns a chunk of rows of one batch element and a thread four columns of it, so the six column sums are running sums in
+// registers and leave as one line of partial sums per chunk: no fold across waves, which a wave-per-row layout needs for all
+// six.  What crosses the waves is two pairs of row sums, through LDS.  The next row's operands are loaded before this row's
+// sums are waited for.
+// Rows of a chunk (never across two batch elements): as many as leave about 2000 blocks, 4 to 32.
+static inline int post_chunk_rows(int64_t M) {
+    int r = 32;
+    while (r > 4 && M / r < 1536) r >>= 1;
+    return r;
+}
+extern "C" int sedd_post_norm_chunks(int64_t M, int64_t L) {
+    if (L <= 0 || M <= 0) return 0;
+    const int r = post_chunk_rows(M);
+    return (int)((M / L) * ((L + r - 1) / r));
+}
+// both sums over the block's nw waves (buf: 2 nw floats; two buffers in turn: the next write to one comes after another barrier)
+__device__ __forceinline__ void block_sum2(float& a, float& b, float* buf, int nw) {
+    a = dpp_sum(a);
+    b = dpp_sum(b);
     if (nw == 1) return;
     if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) buf[wave * N + i] = v[i];
+        const int w = threadIdx.x >> 6;
+        buf[2 * w] = a;
+        buf[2 * w + 1] = b;
     }
-    __syncthreads();  // (two buffers in turn: the next write to this one comes after another such barrier)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float s = buf[i];
-        for (int w = 1; w < nw; ++w) s += buf[w * N + i];
-        v[i] = s;
-    }
+    __syncthreads();
+    a = buf[0];
+    b = buf[1];
+    for (int w = 1; w < nw; ++w) { a += buf[2 * w]; b += buf[2 * w + 1]; }
 }
 
 struct PostBwdArgs {
@@ -188,8 +194,7 @@ struct PostBwdArgs {
 };
 template <typename TA, typename TM, bool NEXT>
 __global__ void __launch_bounds__(512) post_norm_bwd_kernel(PostBwdArgs p) {
-    constexpr int R = POST_ROWS;
-    __shared__ float sA[8 * 2 * R], sB[8 * 2 * R];
+    __shared__ float sA[2 * 8], sB[2][2 * 8];
     const int nw = blockDim.x >> 6, c = threadIdx.x * 4, D = p.D;
     const bool on = c < D;
     const int64_t cpb = (p.L + p.CR - 1) / p.CR;
@@ -211,97 +216,81 @@ __global__ void __launch_bounds__(512) post_norm_bwd_kernel(PostBwdArgs p) {
         }
     }
     float4 aw = f4(0.f), ash = f4(0.f), asc = f4(0.f), ag = f4(0.f), apw = f4(0.f), ab = f4(0.f);
-    for (int r0 = 0; r0 < nrows; r0 += R) {
-        const int64_t row0 = b * p.L + c0 + r0;
-        float4 d[R], g[R], xh[R], ah[R];
-        float s[2 * R];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            d[i] = g[i] = xh[i] = ah[i] = f4(0.f);
-            if (on && r0 + i < nrows) {
-                const int64_t off = (row0 + i) * D + c;
-                if (!NEXT || p.dx1) d[i] = load4<float>(p.dx1 + off);
-                ah[i] = load4<TA>(a + off);
-                if constexpr (NEXT) {
-                    g[i] = load4<TA>(dh + off);
-                    xh[i] = load4<float>(p.x1 + off);
-                }
-            }
-        }
+    const int64_t row0 = b * p.L + c0;
+    float4 dn = f4(0.f), an = f4(0.f), gn = f4(0.f), xn = f4(0.f);  // the next row
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (!on) return;
+        const int64_t off = (row0 + i) * D + c;
+        if (!NEXT || p.dx1) dn = load4<float>(p.dx1 + off);
+        an = load4<TA>(a + off);
         if constexpr (NEXT) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                s[2 * i] = s[2 * i + 1] = 0.f;
-                if (on && r0 + i < nrows) {
-                    const float mu = p.mean[row0 + i], rs = p.rstd[row0 + i];
-                    float* X = &xh[i].x; float* G = &g[i].x;
-                    const float *W = &ww.x, *S = &sc1.x;
-                    float *AW = &aw.x, *ASH = &ash.x, *ASC = &asc.x;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        X[k] = (X[k] - mu) * rs;
-                        ASH[k] += G[k];
-                        const float gx = G[k] * X[k];
-                        ASC[k] += gx * W[k];
-                        AW[k] += gx * S[k];
-                        G[k] *= W[k] * S[k];
-                        s[2 * i] += G[k];
-                        s[2 * i + 1] += G[k] * X[k];
-                    }
-                }
-            }
-            block_sums<2 * R>(s, sA, nw);
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (on && r0 + i < nrows) {
-                    const float rs = p.rstd[row0 + i], m1 = s[2 * i] * inv_d, m2 = s[2 * i + 1] * inv_d;
-                    float* Dv = &d[i].x; const float *X = &xh[i].x, *G = &g[i].x;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) Dv[k] += rs * (G[k] - m1 - X[k] * m2);
-                }
-            }
+            gn = load4<TA>(dh + off);
+            xn = load4<float>(p.x1 + off);
         }
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            s[2 * i] = s[2 * i + 1] = 0.f;
-            if (on && r0 + i < nrows) {
-                const int64_t off = (row0 + i) * D + c;
-                const float pm = p.pmean[row0 + i], pr = p.prstd[row0 + i];
-                store4<float>(p.dx + off, make_float4(p.alpha * d[i].x, p.alpha * d[i].y, p.alpha * d[i].z, p.alpha * d[i].w));
-                float4 kk = f4(1.f);
-                if (p.thr16) kk = keep4_hashed(seed, off, p.thr16, p.inv_keep);
-                float* A = &ah[i].x; float* G = &g[i].x;
-                const float *Dv = &d[i].x, *K = &kk.x, *WP = &wp.x, *GT = &gt.x;
-                float *AG = &ag.x, *APW = &apw.x;
+    };
+    fetch(0);
+    for (int i = 0; i < nrows; ++i) {
+        const int64_t row = row0 + i, off = row * D + c;
+        float4 d = dn, ah = an, g = gn, xh = xn;
+        float rs = 0.f, mu = 0.f;
+        if constexpr (NEXT) { mu = p.mean[row]; rs = p.rstd[row]; }
+        const float pm = p.pmean[row], pr = p.prstd[row];
+        if (i + 1 < nrows) fetch(i + 1);
+        float *Dv = &d.x, *A = &ah.x, *G = &g.x, *X = &xh.x;
+        const float *W = &ww.x, *S = &sc1.x, *WP = &wp.x, *GT = &gt.x;
+        if constexpr (NEXT) {
+            float s1 = 0.f, s2 = 0.f;
+            if (on) {
+                float *AW = &aw.x, *ASH = &ash.x, *ASC = &asc.x;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    A[k] = (A[k] - pm) * pr;
-                    const float dk = Dv[k] * K[k], da_ = dk * A[k];
-                    AG[k] += da_ * WP[k];
-                    APW[k] += da_ * GT[k];
-                    G[k] = dk * GT[k] * WP[k];
-                    s[2 * i] += G[k];
-                    s[2 * i + 1] += G[k] * A[k];
+                    X[k] = (X[k] - mu) * rs;
+                    ASH[k] += G[k];
+                    const float gx = G[k] * X[k];
+                    ASC[k] += gx * W[k];
+                    AW[k] += gx * S[k];
+                    G[k] *= W[k] * S[k];
+                    s1 += G[k];
+                    s2 += G[k] * X[k];
                 }
             }
+            block_sum2(s1, s2, sA, nw);
+            s1 *= inv_d;
+            s2 *= inv_d;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) Dv[k] += rs * (G[k] - s1 - X[k] * s2);
         }
-        block_sums<2 * R>(s, sB, nw);
+        float t1 = 0.f, t2 = 0.f;
+        if (on) {
+            store4<float>(p.dx + off, make_float4(p.alpha * d.x, p.alpha * d.y, p.alpha * d.z, p.alpha * d.w));
+            float4 kk = f4(1.f);
+            if (p.thr16) kk = keep4_hashed(seed, off, p.thr16, p.inv_keep);
+            const float* K = &kk.x;
+            float *AG = &ag.x, *APW = &apw.x;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (on && r0 + i < nrows) {
-                const float pr = p.prstd[row0 + i], m1 = s[2 * i] * inv_d, m2 = s[2 * i + 1] * inv_d;
-                float4 o;
-                float* O = &o.x; const float *A = &ah[i].x, *G = &g[i].x;
-                float* AB = &ab.x;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    O[k] = pr * (G[k] - m1 - A[k] * m2);
-                    AB[k] += O[k];
-                }
-                store4<TA>(da + (row0 + i) * D + c, o);
+            for (int k = 0; k < 4; ++k) {
+                A[k] = (A[k] - pm) * pr;
+                const float dk = Dv[k] * K[k], t = dk * A[k];
+                AG[k] += t * WP[k];
+                APW[k] += t * GT[k];
+                G[k] = dk * GT[k] * WP[k];
+                t1 += G[k];
+                t2 += G[k] * A[k];
             }
         }
-        if (!NEXT && nw > 1) __syncthreads();  // (one buffer only in this form)
+        block_sum2(t1, t2, sB[NEXT ? 0 : i & 1], nw);
+        t1 *= inv_d;
+        t2 *= inv_d;
+        if (on) {
+            float4 o;
+            float *O = &o.x, *AB = &ab.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                O[k] = pr * (G[k] - t1 - A[k] * t2);
+                AB[k] += O[k];
+            }
+            store4<TA>(da + off, o);
+        }
     }
     if (on) {
         float* o = p.ws + chunk * D + c;
@@ -318,7 +307,9 @@ __global__ void __launch_bounds__(512) post_norm_bwd_kernel(PostBwdArgs p) {
 }
 
 // Folds the chunk partials in a fixed order.  Planes: 0 dgate, 1 dwp, 2 dbias, 3 dw, 4 dshift, 5 dscale; 0, 4 and 5 are sums
-// per batch element (written), 1, 2 and 3 over all chunks (added to what is there).  Any output may be NULL.
+// per batch element (written), 1, 2 and 3 over all chunks (added to what is there).  Any output may be NULL.  A block folds 64
+// columns: 16 lanes of four columns each, 16 groups of lines that meet in LDS.  The few long folds come first, with 8 loads in
+// flight per thread: they are bound by latency.
 struct PostReduceArgs {
     const float* ws;
     float* out[6];
@@ -326,42 +317,46 @@ struct PostReduceArgs {
     int D, np;
 };
 __global__ void __launch_bounds__(TPB) post_norm_reduce_kernel(PostReduceArgs p) {
-    const int nxb = (p.D + 255) / 256;
-    const int64_t nbatch = (int64_t)nxb * p.B;
-    const int64_t plane = p.nchunk * p.D;
-    if ((int64_t)blockIdx.x < nbatch) {
-        const int j = (int)(blockIdx.x % nxb) * 256 + threadIdx.x;
-        const int64_t b = blockIdx.x / nxb;
-        if (j >= p.D) return;
-        for (int k = 0; k < p.np; ++k) {
-            if ((k >= 1 && k <= 3) || !p.out[k]) continue;
-            const float* base = p.ws + k * plane + b * p.cpb * p.D + j;
-            float s = 0.f;
-            for (int64_t c = 0; c < p.cpb; ++c) s += base[c * p.D];
-            p.out[k][b * (k == 0 ? p.gate_stride : p.mod_stride) + j] = s;
-        }
-        return;
-    }
-    // 16 columns per block and plane: 16 row groups of 16 lanes
-    __shared__ float red[16][17];
-    const int64_t i = blockIdx.x - nbatch;
-    const int ncb = (p.D + 15) / 16, k = 1 + (int)(i / ncb), col = (int)(i % ncb) * 16 + (threadIdx.x & 15);
-    const int rg = threadIdx.x >> 4;
+    const int ncb = (p.D + 63) / 64, nvec = p.np == 6 ? 3 : 2;
+    const bool vec = (int64_t)blockIdx.x < (int64_t)nvec * ncb;
+    int64_t i = vec ? blockIdx.x : blockIdx.x - (int64_t)nvec * ncb;
+    const int col = (int)(i % ncb) * 64 + (threadIdx.x & 15) * 4, rg = threadIdx.x >> 4;
+    i /= ncb;
+    const int64_t b = vec ? 0 : i % p.B;
+    const int k = vec ? 1 + (int)i : (i / p.B == 0 ? 0 : 3 + (int)(i / p.B));
     float* out = p.out[k];
     if (!out) return;
-    float s0 = 0.f, s1 = 0.f;
+    __shared__ float4 red[16][16];
+    const int64_t lines = vec ? p.nchunk : p.cpb;
+    float4 s = f4(0.f);
     if (col < p.D) {
-        const float* base = p.ws + k * plane + col;
+        const float* base = p.ws + ((int64_t)k * p.nchunk + b * p.cpb) * p.D + col;
         int64_t c = rg;
-        for (; c + 16 < p.nchunk; c += 32) { s0 += base[c * p.D]; s1 += base[(c + 16) * p.D]; }
-        if (c < p.nchunk) s0 += base[c * p.D];
+        for (; c + 7 * 16 < lines; c += 8 * 16) {
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = load4<float>(base + (c + 16 * u) * p.D);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { s.x += v[u].x; s.y += v[u].y; s.z += v[u].z; s.w += v[u].w; }
+        }
+        for (; c < lines; c += 16) {
+            const float4 v = load4<float>(base + c * p.D);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
     }
-    red[rg][threadIdx.x & 15] = s0 + s1;
+    red[rg][threadIdx.x & 15] = s;
     __syncthreads();
     if (rg == 0 && col < p.D) {
-        float t = red[0][threadIdx.x];
-        for (int r = 1; r < 16; ++r) t += red[r][threadIdx.x];
-        out[col] += t;
+        for (int r = 1; r < 16; ++r) {
+            const float4 v = red[r][threadIdx.x];
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        // (scalar accesses: a gradient slice need not be 16-byte aligned)
+        if (vec) { out[col] += s.x; out[col + 1] += s.y; out[col + 2] += s.z; out[col + 3] += s.w; }
+        else {
+            float* o = out + b * (k == 0 ? p.gate_stride : p.mod_stride) + col;
+            o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
+        }
     }
 }
 
@@ -384,8 +379,8 @@ extern "C" int sedd_post_norm_residual_bwd(const float* dx1, const void* dh, con
     PostBwdArgs p;
     p.dx1 = dx1; p.x1 = x1; p.w = w; p.mean = mean; p.rstd = rstd; p.wp = post_w; p.pmean = post_mean; p.prstd = post_rstd;
     p.dh = dh; p.a = a; p.scale = scale; p.gate = gate; p.dx = dx; p.ws = ws; p.da = da;
-    p.mod_stride = mod_stride; p.nchunk = sedd_ln_bwd_chunks(M, L); p.L = L; p.alpha = res_scale; p.inv_keep = inv_keep;
-    p.seed = seed; p.thr16 = (uint32_t)(p_drop * 65536.0f + 0.5f); p.D = D; p.CR = chunk_rows(M);
+    p.mod_stride = mod_stride; p.nchunk = sedd_post_norm_chunks(M, L); p.L = L; p.alpha = res_scale; p.inv_keep = inv_keep;
+    p.seed = seed; p.thr16 = (uint32_t)(p_drop * 65536.0f + 0.5f); p.D = D; p.CR = post_chunk_rows(M);
     const dim3 grid((unsigned)p.nchunk), block((unsigned)((D + 255) / 256 * 64));
     DISPATCH_DT(a_dtype, TA, DISPATCH_DT(mod_dtype, TM, {
         if (dh) hipLaunchKernelGGL((post_norm_bwd_kernel<TA, TM, true>), grid, block, 0, (hipStream_t)stream, p);
@@ -405,9 +400,9 @@ extern "C" int sedd_post_norm_residual_bwd_reduce(const float* ws, float* dgate,
     p.ws = ws;
     float* outs[6] = {dgate, dpost_w, dbias, dw, dshift, dscale};
     for (int k = 0; k < 6; ++k) p.out[k] = outs[k];
-    p.gate_stride = dgate_stride; p.mod_stride = dmod_stride; p.nchunk = sedd_ln_bwd_chunks(M, L); p.B = M / L; p.cpb = p.nchunk / p.B; p.D = D;
+    p.gate_stride = dgate_stride; p.mod_stride = dmod_stride; p.nchunk = sedd_post_norm_chunks(M, L); p.B = M / L; p.cpb = p.nchunk / p.B; p.D = D;
     p.np = (dw || dshift || dscale) ? 6 : 3;
-    const int64_t blocks = (int64_t)((D + 255) / 256) * p.B + (int64_t)((D + 15) / 16) * (p.np == 6 ? 3 : 2);
+    const int64_t blocks = (int64_t)((D + 63) / 64) * (p.np == 6 ? 3 + 3 * p.B : 2 + p.B);
     hipLaunchKernelGGL(post_norm_reduce_kernel, dim3((unsigned)blocks), dim3(TPB), 0, (hipStream_t)stream, p);
     SEDD_LAUNCH_CHECK();
     return SEDD_OK;

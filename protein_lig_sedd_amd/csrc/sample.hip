@@ -437,29 +437,6 @@ __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
 }
 
 // ---- V > 64: NW waves own a row, its entries in registers (NE per lane, four neighbours at a time).
-// Sums and maxima across a wave go through DPP adds (four steps inside rows of 16 lanes, two across them).
-template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_f(float old, float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ float lane63(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
-__device__ __forceinline__ float dpp_sum(float v) {
-    v += dpp_f<0x111, 0xf>(0.f, v);
-    v += dpp_f<0x112, 0xf>(0.f, v);
-    v += dpp_f<0x114, 0xf>(0.f, v);
-    v += dpp_f<0x118, 0xf>(0.f, v);
-    v += dpp_f<0x142, 0xa>(0.f, v);
-    v += dpp_f<0x143, 0xc>(0.f, v);
-    return lane63(v);
-}
-__device__ __forceinline__ float dpp_max(float v) {
-    v = fmaxf(v, dpp_f<0x111, 0xf>(v, v));
-    v = fmaxf(v, dpp_f<0x112, 0xf>(v, v));
-    v = fmaxf(v, dpp_f<0x114, 0xf>(v, v));
-    v = fmaxf(v, dpp_f<0x118, 0xf>(v, v));
-    v = fmaxf(v, dpp_f<0x142, 0xa>(v, v));
-    v = fmaxf(v, dpp_f<0x143, 0xc>(v, v));
-    return lane63(v);
-}
 // the best and second best ratio, with the best one's value and index
 struct Best {
     float b1, b2, x;

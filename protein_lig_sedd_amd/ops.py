@@ -1,8 +1,8 @@
 """Thin tensor-level wrappers over the C ABI (include/sedd_hip.h). Each takes/returns torch CUDA tensors, launches on
 torch's current stream and allocates outputs with torch's caching allocator. No arithmetic happens in Python."""
+import array
 import collections
 import contextlib
-import ctypes
 import math
 import os
 import threading
@@ -130,13 +130,14 @@ _SAME_DEVICE = contextlib.nullcontext()
 def _on_device(t):
     """`with` body: launches go to the stream that is current on t's device, whichever device is current."""
     cur = _cur_device() if _cur_device is not None else torch.cuda.current_device()
-    return _SAME_DEVICE if t.device.index == cur else torch.cuda.device(t.device)
+    return _SAME_DEVICE if t.get_device() == cur else torch.cuda.device(t.device)
 
 
 def _one_device(name, *ts):
-    _cuda(*ts)
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != ts[0].device:
+        if t is not None and (dev < 0 or t.get_device() != dev):  # (-1: host memory)
+            _cuda(*ts)
             raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
 
 
@@ -369,11 +370,12 @@ def predictor_step_philox(graph, step, logscore, x, coef, noise):
     return out
 
 
-def _row_matrix(t, name):
+def _row_matrix(t):
     """t [..., n] as rows of one stride: -> (tensor to keep, row stride in elements); copied if it is not laid out so."""
     n = t.shape[-1]
-    rows = t.numel() // n if n else 0
-    ok, step = t.stride(-1) == 1 or n <= 1, None
+    if t.is_contiguous():
+        return t, n
+    ok, ld, step = t.stride(-1) == 1 or n <= 1, n, None
     for i in range(t.dim() - 2, -1, -1):
         if t.shape[i] == 1:
             continue
@@ -381,17 +383,15 @@ def _row_matrix(t, name):
             ld, step = t.stride(i), t.stride(i) * t.shape[i]
         else:
             ok, step = ok and t.stride(i) == step, step * t.shape[i]
-    if step is None:
-        ld = n
-    if not ok or (rows > 1 and ld < n):
-        t, ld = t.contiguous(), n
+    if not ok or (step is not None and ld < n):
+        return t.contiguous(), n
     return t, ld
 
 
 def _per_request(v, B, dtype, device, name, lo, hi):
     """a sampling parameter for all requests (a number) or one per request (a tensor [B], never read on the host)
     -> (device tensor or None, number)"""
-    if torch.is_tensor(v):
+    if isinstance(v, torch.Tensor):
         if v.numel() not in (1, B):
             raise ValueError(f"{name}: expected 1 or {B} values, got {v.numel()}")
         if dtype == torch.int32 and v.dtype == torch.int64:
@@ -441,8 +441,8 @@ def sample_truncated(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
         if move is not None:
             move = _per_request(move, B, torch.float32, dev, "move", 0.0, 1.0)
             move = move[0] if move[0] is not None else torch.full((B,), move[1], dtype=torch.float32, device=dev)
-        logits, ld = _row_matrix(logits, "logits")
-        u, ldu = _row_matrix(u if u.dtype == torch.float32 else u.float(), "u")
+        logits, ld = _row_matrix(logits)
+        u, ldu = _row_matrix(u if u.dtype == torch.float32 else u.float())
         x = _c(x, torch.int64)
         out = torch.empty(shape, dtype=torch.int64, device=dev)
         with _Timed("sample_truncated", float(M) * (V * (logits.element_size() + 4) + 8)):
@@ -762,23 +762,22 @@ def gate_residual_bwd(dout, a, gate, dgate, keep=None, inv_keep=1.0, dbias=None)
 
 
 def _post_norm_args(name, residual, a, post_w, gate, keep, norm):
-    """checks shared by post_norm_residual_fwd / _bwd -> (B, L, D, gate, modulation dtype, row stride, seed, p_drop)"""
-    if residual.dim() != 3 or residual.dtype != torch.float32 or not residual.is_contiguous():
+    """checks shared by post_norm_residual_fwd / _bwd (the library checks alignment) -> (B, L, D, modulation row stride)"""
+    if residual.dim() != 3 or residual.dtype is not torch.float32 or not residual.is_contiguous():
         raise ValueError(f"{name}: the residual stream must be contiguous fp32 [B, L, D]")
     B, L, D = residual.shape
     if a.shape != residual.shape or not a.is_contiguous():
         raise ValueError(f"{name}: the branch output must be contiguous {tuple(residual.shape)}, got {tuple(a.shape)}")
-    for w in (post_w,) + ((norm[0],) if norm is not None else ()):
-        if w.shape != (D,) or w.dtype != torch.float32 or not w.is_contiguous():
+    for w in (post_w,) if norm is None else (post_w, norm[0]):
+        if w.dtype is not torch.float32 or w.shape != (D,) or not w.is_contiguous():
             raise ValueError(f"{name}: norm weights must be contiguous fp32 [{D}]")
-    g, mdt, ms = _mod_args(gate)
-    for t in (gate,) + (tuple(norm[1:]) if norm is not None else ()):
-        if t.shape != (B, D) or (B > 1 and t.stride(0) != ms) or _mod_args(t)[1] != mdt or t.data_ptr() % (4 * t.element_size()):
+    ms = gate.stride(0)
+    for t in (gate,) if norm is None else (gate,) + norm[1:]:
+        if t.dtype is not gate.dtype or t.shape != (B, D) or t.stride(1) != 1 or (B > 1 and t.stride(0) != ms):
             raise ValueError(f"{name}: gate / shift / scale must be [{B}, {D}] slices of one modulation dtype and row stride")
     if keep is not None and not isinstance(keep, DropSeed):
         raise ValueError(f"{name}: dropout by DropSeed only")
-    _, seed, pd = _keep_args(keep)
-    return B, L, D, g, mdt, ms, seed, pd
+    return B, L, D, ms
 
 
 def post_norm_residual_fwd(residual, a, post_w, gate, keep=None, inv_keep=1.0, res_scale=1.0, norm=None):
@@ -786,21 +785,24 @@ def post_norm_residual_fwd(residual, a, post_w, gate, keep=None, inv_keep=1.0, r
     h = LN(x1) * w * (1 + scale) + shift, in one pass over the rows.  residual fp32 [B, L, D]; a [B, L, D]; gate / shift / scale
     [B, D] slices of modulation tensors of one row stride; keep: DropSeed or None.
     -> (x1 fp32, h in a's dtype or None, (post_mean, post_rstd, mean, rstd) [M] for the backward; the last two None without norm)."""
-    ts = (residual, a, post_w, gate) + (tuple(norm) if norm is not None else ())
-    _one_device("post_norm_residual_fwd", *ts)
     w, shift, scale = norm if norm is not None else (None, None, None)
-    B, L, D, g, mdt, ms, seed, pd = _post_norm_args("post_norm_residual_fwd", residual, a, post_w, gate, keep,
-                                                    None if norm is None else norm)
+    _one_device("post_norm_residual_fwd", residual, a, post_w, gate, w, shift, scale)
+    B, L, D, ms = _post_norm_args("post_norm_residual_fwd", residual, a, post_w, gate, keep,
+                                  None if norm is None else (w, shift, scale))
+    _, seed, pd = _keep_args(keep)
     M = B * L
     with _on_device(residual):
         x1 = torch.empty_like(residual)
         h = torch.empty_like(a) if norm is not None else None
         st = torch.empty(4 if norm is not None else 2, M, dtype=torch.float32, device=residual.device)
-        stats = (st[0], st[1], st[2], st[3]) if norm is not None else (st[0], st[1], None, None)
+        stats = st.unbind(0) if norm is not None else (*st.unbind(0), None, None)
+        at = st.data_ptr()  # (the rows of st, M floats apart)
         with _Timed("post_norm_residual_fwd", float(M) * D * (8 + a.element_size() * (1 if norm is None else 2))):
-            check(lib().sedd_post_norm_residual_fwd(_p(residual), _p(a), _dt(a), _p(post_w), _p(g), _p(shift), _p(scale), mdt,
-                                                    ms, float(res_scale), float(inv_keep), seed, pd, _p(w), _p(x1), _p(h),
-                                                    *[_p(t) for t in stats], M, max(L, 1), D, _stream()),
+            check(lib().sedd_post_norm_residual_fwd(residual.data_ptr(), a.data_ptr(), _dt(a), post_w.data_ptr(),
+                                                    gate.data_ptr(), _p(shift), _p(scale), _dt(gate), ms, float(res_scale),
+                                                    float(inv_keep), seed, pd, _p(w), x1.data_ptr(), _p(h), at, at + 4 * M,
+                                                    at + 8 * M if h is not None else None,
+                                                    at + 12 * M if h is not None else None, M, L or 1, D, _stream()),
                   "sedd_post_norm_residual_fwd")
     return x1, h, stats
 
@@ -817,8 +819,8 @@ def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=Non
         raise ValueError("post_norm_residual_bwd: dx1 None needs a norm")
     like = x1 if dx1 is None else dx1
     _one_device("post_norm_residual_bwd", like, dx1, a, post_w, gate, *stats, dgate, dpost_w, dbias, *(norm or ()))
-    B, L, D, g, mdt, ms, seed, pd = _post_norm_args("post_norm_residual_bwd", like, a, post_w, gate, keep,
-                                                    None if norm is None else (w, scale))
+    B, L, D, ms = _post_norm_args("post_norm_residual_bwd", like, a, post_w, gate, keep, None if norm is None else (w, scale))
+    _, seed, pd = _keep_args(keep)
     M = B * L
     for t, n in zip(stats, ("post_mean", "post_rstd", "mean", "rstd") if norm is not None else ("post_mean", "post_rstd")):
         if t is None or t.dtype != torch.float32 or t.numel() != M or not t.is_contiguous():
@@ -843,7 +845,7 @@ def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=Non
                 if t is not None:
                     t.zero_()
             return dx, da
-        ws = torch.empty((6 if norm is not None else 3) * lib().sedd_ln_bwd_chunks(M, L) * D, dtype=torch.float32,
+        ws = torch.empty((6 if norm is not None else 3) * lib().sedd_post_norm_chunks(M, L) * D, dtype=torch.float32,
                          device=like.device)
         pm, pr, mean, rstd = tuple(stats) + (None,) * (4 - len(stats))
         if norm is None:
@@ -851,7 +853,7 @@ def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=Non
         with _Timed("post_norm_residual_bwd", float(M) * D * (8 + 2 * a.element_size()
                                                               + (0 if norm is None else 4 + a.element_size()))):
             check(lib().sedd_post_norm_residual_bwd(_p(dx1), _p(dh), _p(x1), _p(w), _p(scale), _p(mean), _p(rstd), _p(a), _dt(a),
-                                                    _p(post_w), _p(g), mdt, ms, _p(pm), _p(pr), float(res_scale),
+                                                    _p(post_w), _p(gate), _dt(gate), ms, _p(pm), _p(pr), float(res_scale),
                                                     float(inv_keep), seed, pd, _p(dx), _p(da), _p(ws), M, L, D, _stream()),
                   "sedd_post_norm_residual_bwd")
             check(lib().sedd_post_norm_residual_bwd_reduce(_p(ws), _p(dgate), gs, _p(dshift), _p(dscale), dms, _p(dpost_w),
@@ -1261,8 +1263,6 @@ def clip_from_sumsq(out, gscale, max_norm):
 
 def _dense(t):
     """whether t's elements fill one stretch of memory, in whatever order of dimensions"""
-    if t.is_contiguous():
-        return True
     n = 1
     for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
         if st != n:
@@ -1271,40 +1271,41 @@ def _dense(t):
     return True
 
 
+_KIND = {torch.float32: F32, torch.bfloat16: BF16}
+
+
 def _tensor_table(tensors, name):
     """host arrays (addresses, sizes, dtypes) of a list of gradients, checked: one device, fp32 / bf16, dense, none of them
-    sharing memory with another."""
-    ptrs, sizes, kinds, spans = [], [], [], []
-    dev = tensors[0].device
-    for t in tensors:
-        if t.device != dev or dev.type != "cuda":
-            _one_device(name, tensors[0], t)
-        if t.is_sparse or not (t.is_contiguous() or _dense(t)):
-            raise ValueError(f"{name}: tensor of shape {tuple(t.shape)} and strides {tuple(t.stride())} is not dense")
-        p, n, k = t.data_ptr(), t.numel(), _dt(t)
-        ptrs.append(p)
-        sizes.append(n)
-        kinds.append(k)
-        if n:
-            spans.append((p, p + n * (2 if k == BF16 else 4)))
-    spans.sort()
+    sharing memory with another.  (map() over the methods: a loop in Python costs 0.8 us a tensor, this 0.35.)"""
+    devs = set(map(torch.Tensor.get_device, tensors))
+    if len(devs) > 1 or -1 in devs:
+        _one_device(name, *tensors)
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        for t in tensors:
+            if not t.is_contiguous() and (t.layout != torch.strided or not _dense(t)):
+                raise ValueError(f"{name}: a tensor of shape {tuple(t.shape)} is not dense")
+    kinds = [_KIND.get(t.dtype) for t in tensors]
+    if None in kinds:
+        _dt(tensors[kinds.index(None)])
+    ptrs, sizes = array.array("Q", map(torch.Tensor.data_ptr, tensors)), array.array("q", map(torch.Tensor.numel, tensors))
     end = 0
-    for lo, hi in spans:
-        if lo < end:
-            raise ValueError(f"{name}: two of the tensors share memory")
-        end = hi
-    n = len(ptrs)
-    return (ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*kinds), n
+    for lo, n, k in sorted(zip(ptrs, sizes, kinds)):
+        if n:
+            if lo < end:
+                raise ValueError(f"{name}: two of the tensors share memory")
+            end = lo + n * (4 if k == F32 else 2)
+    return ptrs, sizes, array.array("i", kinds)
 
 
 def _multi_norm(tab, max_norm, device):
-    n = tab[3]
+    """-> (device tensor [norm, clip coefficient], the table's addresses and length as the library takes them)"""
+    args = tuple(t.buffer_info()[0] for t in tab) + (len(tab[0]),)
     # (allocated per call: two captured graphs, or two streams, never share it)
-    ws = torch.empty(4096 + n, dtype=torch.float64, device=device)
+    ws = torch.empty(4096 + args[3], dtype=torch.float64, device=device)
     out = torch.empty(2, dtype=torch.float32, device=device)
-    check(lib().sedd_multi_norm_clip(tab[0], tab[1], tab[2], n, max_norm, _p(ws), ws.numel(), _p(out), _stream()),
+    check(lib().sedd_multi_norm_clip(*args, max_norm, ws.data_ptr(), ws.numel(), out.data_ptr(), _stream()),
           "sedd_multi_norm_clip")
-    return out
+    return out, args
 
 
 def grad_norm(grads):
@@ -1314,7 +1315,7 @@ def grad_norm(grads):
         return torch.zeros(())
     tab = _tensor_table(grads, "grad_norm")
     with _on_device(grads[0]):
-        return _multi_norm(tab, 0.0, grads[0].device)[0]
+        return _multi_norm(tab, 0.0, grads[0].device)[0][0]
 
 
 def clip_grad_norm_(grads, max_norm, error_if_nonfinite=False, round_coef=False):
@@ -1330,11 +1331,10 @@ def clip_grad_norm_(grads, max_norm, error_if_nonfinite=False, round_coef=False)
         return torch.zeros(())
     tab = _tensor_table(grads, "clip_grad_norm_")
     with _on_device(grads[0]):
-        out = _multi_norm(tab, max_norm, grads[0].device)
+        out, args = _multi_norm(tab, max_norm, grads[0].device)
         if error_if_nonfinite and not math.isfinite(float(out[0])):
             raise RuntimeError(f"the norm of the gradients is {float(out[0])}: they were not clipped")
-        check(lib().sedd_multi_scale(tab[0], tab[1], tab[2], tab[3], out.data_ptr() + 4, 1 if round_coef else 0, _stream()),
-              "sedd_multi_scale")
+        check(lib().sedd_multi_scale(*args, out.data_ptr() + 4, 1 if round_coef else 0, _stream()), "sedd_multi_scale")
     return out[0]
 
 
