@@ -47,7 +47,7 @@ SIGNATURES = {
     "sedd_gate_residual_bwd": "ppipilpflfppillip",
     "sedd_gate_residual_bwd_reduce": "pplp" + "llip",
     "sedd_gate_residual_ln_modulate_fwd": "ppipppil" + "flf" + "ppppp" + "llip",
-    "sedd_post_norm_chunks": "ll",
+    "sedd_post_norm_chunks": "lli",
     "sedd_post_norm_residual_fwd": "ppipppp" + "il" + "fflf" + "ppp" + "pppp" + "llip",
     "sedd_post_norm_residual_bwd": "ppppppp" + "pipp" + "ilpp" + "fflf" + "ppp" + "llip",
     "sedd_post_norm_residual_bwd_reduce": "pplppl" + "ppp" + "llip",

@@ -154,15 +154,18 @@ extern "C" int sedd_post_norm_residual_fwd(const float* residual, const void* a,
 // registers and leave as one line of partial sums per chunk: no fold across waves, which a wave-per-row layout needs for all
 // six.  What crosses the waves is two pairs of row sums, through LDS.  The next row's operands are loaded before this row's
 // sums are waited for.
-// Rows of a chunk (never across two batch elements): as many as leave about 2000 blocks, 4 to 32.
-static inline int post_chunk_rows(int64_t M) {
+// Rows of a chunk (never across two batch elements): 32, or fewer where that leaves less than 2560 waves (10 a CU).  Measured with
+// half and twice the rows: 64 x 512 x 768 32 rows 113 us (16: 121, 64: 155); 16 x 1024 x 1024 16 rows 71 (8: 80, 32: 86);
+// 8 x 512 x 2048 8 rows 36 (4: 46); more waves cover the latency of the row sums, more chunks write more partial sums.
+static inline int post_chunk_rows(int64_t M, int D) {
+    const int64_t nw = (D + 255) / 256;
     int r = 32;
-    while (r > 4 && M / r < 1536) r >>= 1;
+    while (r > 4 && M / r * nw < 2560) r >>= 1;
     return r;
 }
-extern "C" int sedd_post_norm_chunks(int64_t M, int64_t L) {
+extern "C" int sedd_post_norm_chunks(int64_t M, int64_t L, int D) {
     if (L <= 0 || M <= 0) return 0;
-    const int r = post_chunk_rows(M);
+    const int r = post_chunk_rows(M, D);
     return (int)((M / L) * ((L + r - 1) / r));
 }
 // both sums over the block's nw waves (buf: 2 nw floats; two buffers in turn: the next write to one comes after another barrier)
@@ -379,8 +382,8 @@ extern "C" int sedd_post_norm_residual_bwd(const float* dx1, const void* dh, con
     PostBwdArgs p;
     p.dx1 = dx1; p.x1 = x1; p.w = w; p.mean = mean; p.rstd = rstd; p.wp = post_w; p.pmean = post_mean; p.prstd = post_rstd;
     p.dh = dh; p.a = a; p.scale = scale; p.gate = gate; p.dx = dx; p.ws = ws; p.da = da;
-    p.mod_stride = mod_stride; p.nchunk = sedd_post_norm_chunks(M, L); p.L = L; p.alpha = res_scale; p.inv_keep = inv_keep;
-    p.seed = seed; p.thr16 = (uint32_t)(p_drop * 65536.0f + 0.5f); p.D = D; p.CR = post_chunk_rows(M);
+    p.mod_stride = mod_stride; p.nchunk = sedd_post_norm_chunks(M, L, D); p.L = L; p.alpha = res_scale; p.inv_keep = inv_keep;
+    p.seed = seed; p.thr16 = (uint32_t)(p_drop * 65536.0f + 0.5f); p.D = D; p.CR = post_chunk_rows(M, D);
     const dim3 grid((unsigned)p.nchunk), block((unsigned)((D + 255) / 256 * 64));
     DISPATCH_DT(a_dtype, TA, DISPATCH_DT(mod_dtype, TM, {
         if (dh) hipLaunchKernelGGL((post_norm_bwd_kernel<TA, TM, true>), grid, block, 0, (hipStream_t)stream, p);
@@ -400,7 +403,7 @@ extern "C" int sedd_post_norm_residual_bwd_reduce(const float* ws, float* dgate,
     p.ws = ws;
     float* outs[6] = {dgate, dpost_w, dbias, dw, dshift, dscale};
     for (int k = 0; k < 6; ++k) p.out[k] = outs[k];
-    p.gate_stride = dgate_stride; p.mod_stride = dmod_stride; p.nchunk = sedd_post_norm_chunks(M, L); p.B = M / L; p.cpb = p.nchunk / p.B; p.D = D;
+    p.gate_stride = dgate_stride; p.mod_stride = dmod_stride; p.nchunk = sedd_post_norm_chunks(M, L, D); p.B = M / L; p.cpb = p.nchunk / p.B; p.D = D;
     p.np = (dw || dshift || dscale) ? 6 : 3;
     const int64_t blocks = (int64_t)((D + 63) / 64) * (p.np == 6 ? 3 + 3 * p.B : 2 + p.B);
     hipLaunchKernelGGL(post_norm_reduce_kernel, dim3((unsigned)blocks), dim3(TPB), 0, (hipStream_t)stream, p);

@@ -160,22 +160,135 @@ __device__ __forceinline__ Verdict judge(const RowParams& rp, int rank, float S,
 }
 
 // ------------------------------------------------------------------------------- the definition itself, in 64 bits
-// Reads the row again in every pass: for rows that came near, for rows outside the range of the 32-bit bounds, and for rows too
-// long for registers; xs: LDS for the scores of a row, if it fits.  Within that range the arg-max is looked for among the entries whose 32-bit ratio comes within twice the
-// tolerance of the largest, usually one or two, and only those are evaluated in 64 bits.
+// Three forms.  A wave with an entry per lane (V <= 64): the rank of every entry and the mass before it in one loop over the
+// lanes, then the arg-max over what is kept.
+template <typename T> __device__ int64_t resolve_lanes64(const SampleArgs& a, int64_t row, int64_t b) {
+    const int lane = threadIdx.x & 63;
+    const RowParams rp = row_params(a, b);
+    const float v = lane < a.V ? to_f32<T>(((const T*)a.x + row * a.ld)[lane]) + 0.0f : -INFINITY;
+    const float u = lane < a.V ? (a.u + row * a.ldu)[lane] : 0.5f;
+    const bool in = v > -INFINITY;
+    const float mx = dpp_max(in ? v : -INFINITY);
+    if (!(mx > -INFINITY)) return row_empty(a);
+    if (!(rp.T > 0.f)) return __builtin_ctzll(__ballot(v == mx));  // greedy
+    const double q = !in ? 0.0 : v == mx ? 1.0 : mx == INFINITY ? 0.0 : exp(((double)v - (double)mx) / (double)rp.T);
+    const double r = in ? q / (1e-10 - log((double)noise_arg(u))) : -1.0;
+    int rank = 0;
+    double S = 0.0;
+    for (int i = 0; i < a.V; ++i) {
+        const float vi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+        const int lo = __builtin_amdgcn_readlane((int)__double2loint(q), i), hi = __builtin_amdgcn_readlane((int)__double2hiint(q), i);
+        if ((vi > v) | ((vi == v) & (i < lane))) {  // (false for NaN)
+            ++rank;
+            S += __hiloint2double(hi, lo);
+        }
+    }
+    double W = rank < rp.k ? q : 0.0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) W += __shfl_xor(W, o, 64);
+    const bool kept = in && (rank == 0 || (rank < rp.k && (!(rp.P < 1.f) || S < (double)rp.P * W) && !(q < (double)rp.m)));
+    double best = kept ? r : -1.0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const double other = __shfl_xor(best, o, 64);
+        best = other > best ? other : best;
+    }
+    return __builtin_ctzll(__ballot(kept && r == best));
+}
+// A block with the row's scores, weights and ratios in LDS (V <= STAGED).
+#define STAGED 4096
+struct StagedRow {
+    double q[STAGED], r[STAGED];
+    float x[STAGED];
+};
 template <typename T, int NT>
-__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, double* sd, int64_t* si, float* xs = nullptr) {
+__device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b, StagedRow& s, double* sd, int64_t* si) {
     Joint<NT> J{sd, si};
     const int lane = threadIdx.x & (NT - 1), V = a.V;
     const T* px = (const T*)a.x + row * a.ld;
     const float* u = a.u + row * a.ldu;
-    if (xs) {
-        __syncthreads();
-#pragma unroll 4
-        for (int j = lane; j < V; j += NT) xs[j] = to_f32<T>(px[j]);
-        __syncthreads();
+    const RowParams rp = row_params(a, b);
+    const int64_t none = (int64_t)1 << 40;
+    __syncthreads();
+    double top = -1.0;  // (an order key, so that one reduction serves)
+    int64_t mi = none;
+    for (int j = lane; j < V; j += NT) {
+        const float v = to_f32<T>(px[j]);
+        const uint32_t key = order_key(v);
+        s.x[j] = key ? v : -INFINITY;
+        if (key && (double)key > top) { top = (double)key; mi = j; }
     }
-    auto score = [&](int64_t j) { return xs ? xs[j] : to_f32<T>(px[j]); };
+    J.best(top, mi);
+    if (mi == none) return row_empty(a);
+    if (!(rp.T > 0.f)) return mi;  // greedy
+    const float mx = s.x[mi];
+    for (int j = lane; j < V; j += NT) {
+        const float v = s.x[j];
+        const double q = v == mx ? 1.0 : !(v > -INFINITY) || mx == INFINITY ? 0.0 : exp(((double)v - (double)mx) / (double)rp.T);
+        s.q[j] = q;
+        s.r[j] = v > -INFINITY ? q / (1e-10 - log((double)noise_arg(u[j]))) : -1.0;
+    }
+    double W = 0.0;
+    if (rp.P < 1.f) {
+        uint32_t t = 0;  // the k-th largest key, or 0 if there are no k candidates
+        for (int bit = 31; rp.k < V && bit >= 0; --bit) {
+            const uint32_t ct = t | (1u << bit);
+            int64_t n = 0;
+            for (int j = lane; j < V; j += NT) n += order_key(s.x[j]) >= ct;
+            n = J.isum(n);
+            if (n >= rp.k) t = ct;
+            if (n == rp.k) break;  // (then exactly the k first are at or above t)
+        }
+        double border = 0.0;
+        int64_t n = 0, any = 0;
+        for (int j = lane; j < V; j += NT) {
+            const uint32_t key = order_key(s.x[j]);
+            if (key > t) { W += s.q[j]; ++n; }
+            else if (key == t && t) border = s.q[j];
+        }
+        W = J.sum(W);
+        if (t) {
+            n = J.isum(n);
+            J.best(border, any);
+            W += (double)(rp.k - n) * border;  // of equal entries at the border the lowest indices are in; they weigh the same
+        }
+    }
+    float cx = -INFINITY;  // what is still possible: ranked before (cx, ci); at first all
+    int64_t ci = -1;
+    for (;;) {
+        double best = -1.0;
+        int64_t bi = none;
+        for (int j = lane; j < V; j += NT) {
+            const float v = s.x[j];
+            if (s.r[j] > best && (v > cx || (v == cx && j < ci))) { best = s.r[j]; bi = j; }
+        }
+        J.best(best, bi);
+        if (bi == none) return mi;  // (cannot be: the first of the order is always kept)
+        const float vw = s.x[bi];
+        int64_t rank = 0;
+        double S = 0.0;
+        for (int j = lane; j < V; j += NT) {
+            const float v = s.x[j];
+            if (v > vw || (v == vw && j < bi)) { S += s.q[j]; ++rank; }
+        }
+        rank = J.isum(rank);
+        if (rank == 0) return bi;
+        S = J.sum(S);
+        if (rank < rp.k && (!(rp.P < 1.f) || S < (double)rp.P * W) && !(s.q[bi] < (double)rp.m)) return bi;
+        cx = vw;
+        ci = bi;
+    }
+}
+// Threads that read the row again in every pass, for any V.  Within the range of the 32-bit bounds the arg-max is looked for among
+// the entries whose 32-bit ratio comes within twice the tolerance of the largest, usually one or two, and only those are
+// evaluated in 64 bits.
+template <typename T, int NT>
+__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, double* sd, int64_t* si) {
+    Joint<NT> J{sd, si};
+    const int lane = threadIdx.x & (NT - 1), V = a.V;
+    const T* px = (const T*)a.x + row * a.ld;
+    const float* u = a.u + row * a.ldu;
+    auto score = [&](int64_t j) { return to_f32<T>(px[j]); };
     const RowParams rp = row_params(a, b);
     const int64_t none = (int64_t)1 << 40;
     // the first entry of the order
@@ -430,7 +543,7 @@ __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
     for (unsigned long long todo = __ballot(near); todo; todo &= todo - 1) {
         const int src = __builtin_ctzll(todo);
         const int rr = __builtin_amdgcn_readlane(on ? r : 0, src);
-        const int64_t v = resolve_row64<T, 64>(a, row0 + rr, batch_of(rr), nullptr, nullptr);
+        const int64_t v = resolve_lanes64<T>(a, row0 + rr, batch_of(rr));
         if (lane == src) ans = v;
     }
     if (on) a.out[row] = ans;
@@ -801,7 +914,6 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
 // kernel, the 64-bit arithmetic would take its registers (115 instead of 60) and half of its waves (131072 x 300: 159 us with it,
 // 79 us and 4 us for the launch behind without), and one wave alone with a row would be the last of the launch by 50 us.
 #define NEAR_TOKEN INT64_MIN
-#define NEAR_ROW 12288
 template <typename T, int NW, int NE>
 __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sample_wide_kernel(SampleArgs a) {
     __shared__ WideShared<NW> sh;
@@ -814,11 +926,10 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sam
     if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN : ans;
 }
 // a block looks through `per` rows (at most 256) and takes those that came near one after the other
-template <typename T> __global__ void __launch_bounds__(256) sample_near_kernel(SampleArgs a, int per) {
+template <typename T, bool FITS> __global__ void __launch_bounds__(256) sample_near_kernel(SampleArgs a, int per) {
     __shared__ double sd[4];
     __shared__ int64_t si[4];
     __shared__ uint64_t s_mask[4];
-    __shared__ float s_row[NEAR_ROW];
     const int64_t row0 = (int64_t)blockIdx.x * per, mine = row0 + threadIdx.x;
     const bool near = (int)threadIdx.x < per && mine < a.M && a.out[mine] == NEAR_TOKEN;
     const uint64_t mask = __ballot(near);
@@ -826,8 +937,14 @@ template <typename T> __global__ void __launch_bounds__(256) sample_near_kernel(
     __syncthreads();
     for (int w = 0; w < 4; ++w) {
         for (uint64_t todo = s_mask[w]; todo; todo &= todo - 1) {
-            const int64_t row = row0 + w * 64 + __builtin_ctzll(todo);
-            const int64_t ans = resolve_row64<T, 256>(a, row, batch_of_row(a, row), sd, si, a.V <= NEAR_ROW ? s_row : nullptr);
+            const int64_t row = row0 + w * 64 + __builtin_ctzll(todo), b = batch_of_row(a, row);
+            int64_t ans;
+            if constexpr (FITS) {
+                __shared__ StagedRow s_row;
+                ans = resolve_staged64<T, 256>(a, row, b, s_row, sd, si);
+            } else {
+                ans = resolve_row64<T, 256>(a, row, b, sd, si);
+            }
             if (threadIdx.x == 0) a.out[row] = ans;
         }
     }
@@ -852,9 +969,11 @@ template <typename T, int VP> static void launch_lane(const SampleArgs& a, hipSt
 template <typename T, int NW, int NE> static void launch_wide(const SampleArgs& a, hipStream_t st) {
     constexpr int R = NW == 1 ? 4 : 1;
     hipLaunchKernelGGL((sample_wide_kernel<T, NW, NE>), dim3((unsigned)((a.M + R - 1) / R)), dim3(NW == 1 ? 256 : NW * 64), 0, st, a);
-    int64_t per = (a.M + 2047) / 2048;
+    int64_t per = (a.M + 511) / 512;  // (a block of the staged form fills half of a CU's LDS: two rounds of blocks at most)
     per = per > 256 ? 256 : per;
-    hipLaunchKernelGGL((sample_near_kernel<T>), dim3((unsigned)((a.M + per - 1) / per)), dim3(256), 0, st, a, (int)per);
+    const dim3 grid((unsigned)((a.M + per - 1) / per));
+    if (a.V <= STAGED) hipLaunchKernelGGL((sample_near_kernel<T, true>), grid, dim3(256), 0, st, a, (int)per);
+    else hipLaunchKernelGGL((sample_near_kernel<T, false>), grid, dim3(256), 0, st, a, (int)per);
 }
 template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t st) {
     // V up to a multiple of 4 (8 above 32): the entries behind V cost arithmetic, and a row is never read past its end

@@ -845,7 +845,7 @@ def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=Non
                 if t is not None:
                     t.zero_()
             return dx, da
-        ws = torch.empty((6 if norm is not None else 3) * lib().sedd_post_norm_chunks(M, L) * D, dtype=torch.float32,
+        ws = torch.empty((6 if norm is not None else 3) * lib().sedd_post_norm_chunks(M, L, D) * D, dtype=torch.float32,
                          device=like.device)
         pm, pr, mean, rstd = tuple(stats) + (None,) * (4 - len(stats))
         if norm is None:
