@@ -195,14 +195,15 @@ template <typename T> __device__ int64_t resolve_lanes64(const SampleArgs& a, in
     }
     return __builtin_ctzll(__ballot(kept && r == best));
 }
-// A block with the row's scores, weights and ratios in LDS (V <= STAGED).
+// A block with the row's scores, weights and ratios in LDS (V <= STAGED).  kth: what kth_key has found for the row, 0 if it is
+// not known (the search for it in here costs more than all the rest: 20 us of 40 at V = 2365).
 #define STAGED 4096
 struct StagedRow {
     double q[STAGED], r[STAGED];
     float x[STAGED];
 };
 template <typename T, int NT>
-__device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b, StagedRow& s, double* sd, int64_t* si) {
+__device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b, uint32_t kth, StagedRow& s, double* sd, int64_t* si) {
     Joint<NT> J{sd, si};
     const int lane = threadIdx.x & (NT - 1), V = a.V;
     const T* px = (const T*)a.x + row * a.ld;
@@ -230,8 +231,8 @@ __device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b,
     }
     double W = 0.0;
     if (rp.P < 1.f) {
-        uint32_t t = 0;  // the k-th largest key, or 0 if there are no k candidates
-        for (int bit = 31; rp.k < V && bit >= 0; --bit) {
+        uint32_t t = kth;  // the k-th largest key, or 0 if there are no k candidates
+        for (int bit = 31; !kth && rp.k < V && bit >= 0; --bit) {
             const uint32_t ct = t | (1u << bit);
             int64_t n = 0;
             for (int j = lane; j < V; j += NT) n += order_key(s.x[j]) >= ct;
@@ -283,7 +284,7 @@ __device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b,
 // the entries whose 32-bit ratio comes within twice the tolerance of the largest, usually one or two, and only those are
 // evaluated in 64 bits.
 template <typename T, int NT>
-__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, double* sd, int64_t* si) {
+__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, uint32_t kth, double* sd, int64_t* si) {
     Joint<NT> J{sd, si};
     const int lane = threadIdx.x & (NT - 1), V = a.V;
     const T* px = (const T*)a.x + row * a.ld;
@@ -317,8 +318,8 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, do
     // mass of the k first of the order (when it is needed)
     double W = -1.0;
     auto mass = [&]() {
-        uint32_t t = 0;
-        if (rp.k < V) {  // the k-th largest key; 0 if there are no k candidates
+        uint32_t t = kth;
+        if (!kth && rp.k < V) {  // the k-th largest key; 0 if there are no k candidates
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t ct = t | (1u << bit);
                 int64_t n = 0;
@@ -747,9 +748,9 @@ template <int NW> struct WideShared {
     float red[2][4 * NW];
     int n, ans;
 };
-// the token of a row that is sampled; near: it is not settled
+// the token of a row that is sampled; near: it is not settled; t: the k-th key if it was needed, else 0 (wave 0's is meant)
 template <typename T, int NW, int NE>
-__device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, int64_t b, WideShared<NW>& sh, bool& near) {
+__device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, int64_t b, WideShared<NW>& sh, bool& near, uint32_t& t) {
     constexpr int NT = NW * 64, LOW = sizeof(T) == 2 ? 16 : 0;
     const int V = a.V, lane = threadIdx.x & 63, tid = NW == 1 ? lane : (int)threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), slot = NW == 1 ? wave : 0;
@@ -812,7 +813,6 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
             if (!near) {
                 // a bound that what is kept reaches
                 float thr = -INFINITY;
-                uint32_t t = 0;
                 int n = PACK + 1;
                 auto reach = [&]() __attribute__((always_inline)) {
                     int m = 0;
@@ -910,7 +910,7 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
     }
 }
 
-// A row that came near gets this in place of its token until sample_near_kernel, launched behind, has decided it: kept in this
+// A row that came near gets this, and its k-th key in the low half, in place of its token until sample_near_kernel, launched behind, has decided it: kept in this
 // kernel, the 64-bit arithmetic would take its registers (115 instead of 60) and half of its waves (131072 x 300: 159 us with it,
 // 79 us and 4 us for the launch behind without), and one wave alone with a row would be the last of the launch by 50 us.
 #define NEAR_TOKEN INT64_MIN
@@ -922,28 +922,33 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sam
     if (row >= a.M) return;
     const int64_t b = batch_of_row(a, row);
     bool near = false;
-    const int64_t ans = row_moves(a, row, b) ? wide_row<T, NW, NE>(a, row, b, sh, near) : a.xcur[row];
-    if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN : ans;
+    uint32_t t = 0;
+    const int64_t ans = row_moves(a, row, b) ? wide_row<T, NW, NE>(a, row, b, sh, near, t) : a.xcur[row];
+    if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN + (int64_t)t : ans;
 }
 // a block looks through `per` rows (at most 256) and takes those that came near one after the other
 template <typename T, bool FITS> __global__ void __launch_bounds__(256) sample_near_kernel(SampleArgs a, int per) {
     __shared__ double sd[4];
     __shared__ int64_t si[4];
     __shared__ uint64_t s_mask[4];
+    __shared__ uint32_t s_kth[256];
     const int64_t row0 = (int64_t)blockIdx.x * per, mine = row0 + threadIdx.x;
-    const bool near = (int)threadIdx.x < per && mine < a.M && a.out[mine] == NEAR_TOKEN;
+    const int64_t got = (int)threadIdx.x < per && mine < a.M ? a.out[mine] : 0;
+    const bool near = got < NEAR_TOKEN + ((int64_t)1 << 32) && row_moves(a, mine, batch_of_row(a, mine));
     const uint64_t mask = __ballot(near);
     if ((threadIdx.x & 63) == 0) s_mask[threadIdx.x >> 6] = mask;
+    s_kth[threadIdx.x] = (uint32_t)got;
     __syncthreads();
     for (int w = 0; w < 4; ++w) {
         for (uint64_t todo = s_mask[w]; todo; todo &= todo - 1) {
             const int64_t row = row0 + w * 64 + __builtin_ctzll(todo), b = batch_of_row(a, row);
+            const uint32_t kth = s_kth[row - row0];
             int64_t ans;
             if constexpr (FITS) {
                 __shared__ StagedRow s_row;
-                ans = resolve_staged64<T, 256>(a, row, b, s_row, sd, si);
+                ans = resolve_staged64<T, 256>(a, row, b, kth, s_row, sd, si);
             } else {
-                ans = resolve_row64<T, 256>(a, row, b, sd, si);
+                ans = resolve_row64<T, 256>(a, row, b, kth, sd, si);
             }
             if (threadIdx.x == 0) a.out[row] = ans;
         }
@@ -958,7 +963,7 @@ __global__ void __launch_bounds__(NT) sample_row64_kernel(SampleArgs a) {
         const int64_t b = batch_of_row(a, row);
         int64_t got;
         if (!row_moves(a, row, b)) got = a.xcur[row];
-        else got = resolve_row64<T, NT>(a, row, b, sd, si);
+        else got = resolve_row64<T, NT>(a, row, b, 0, sd, si);
         if (threadIdx.x == 0) a.out[row] = got;
     }
 }
