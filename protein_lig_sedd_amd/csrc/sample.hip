@@ -927,11 +927,15 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sam
     if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN + (int64_t)t : ans;
 }
 // a block looks through `per` rows (at most 256) and takes those that came near one after the other
-template <typename T, bool FITS> __global__ void __launch_bounds__(256) sample_near_kernel(SampleArgs a, int per) {
-    __shared__ double sd[4];
-    __shared__ int64_t si[4];
-    __shared__ uint64_t s_mask[4];
-    __shared__ uint32_t s_kth[256];
+// 512 threads to a row: of one near row the launch takes 7.5 us at V = 2365 and 21 us at V = 9000 (256 threads: 9.5 and 29,
+// 1024: 12 and 21; and where no row is near, 4 us against 4 and 7)
+#define NEAR_NT 512
+template <typename T, bool FITS> __global__ void __launch_bounds__(NEAR_NT) sample_near_kernel(SampleArgs a, int per) {
+    constexpr int NT = NEAR_NT;
+    __shared__ double sd[NT / 64];
+    __shared__ int64_t si[NT / 64];
+    __shared__ uint64_t s_mask[NT / 64];
+    __shared__ uint32_t s_kth[NT];
     const int64_t row0 = (int64_t)blockIdx.x * per, mine = row0 + threadIdx.x;
     const int64_t got = (int)threadIdx.x < per && mine < a.M ? a.out[mine] : 0;
     const bool near = got < NEAR_TOKEN + ((int64_t)1 << 32) && row_moves(a, mine, batch_of_row(a, mine));
@@ -946,9 +950,9 @@ template <typename T, bool FITS> __global__ void __launch_bounds__(256) sample_n
             int64_t ans;
             if constexpr (FITS) {
                 __shared__ StagedRow s_row;
-                ans = resolve_staged64<T, 256>(a, row, b, kth, s_row, sd, si);
+                ans = resolve_staged64<T, NT>(a, row, b, kth, s_row, sd, si);
             } else {
-                ans = resolve_row64<T, 256>(a, row, b, kth, sd, si);
+                ans = resolve_row64<T, NT>(a, row, b, kth, sd, si);
             }
             if (threadIdx.x == 0) a.out[row] = ans;
         }
@@ -977,8 +981,8 @@ template <typename T, int NW, int NE> static void launch_wide(const SampleArgs& 
     int64_t per = (a.M + 511) / 512;  // (a block of the staged form fills half of a CU's LDS: two rounds of blocks at most)
     per = per > 256 ? 256 : per;
     const dim3 grid((unsigned)((a.M + per - 1) / per));
-    if (a.V <= STAGED) hipLaunchKernelGGL((sample_near_kernel<T, true>), grid, dim3(256), 0, st, a, (int)per);
-    else hipLaunchKernelGGL((sample_near_kernel<T, false>), grid, dim3(256), 0, st, a, (int)per);
+    if (a.V <= STAGED) hipLaunchKernelGGL((sample_near_kernel<T, true>), grid, dim3(NEAR_NT), 0, st, a, (int)per);
+    else hipLaunchKernelGGL((sample_near_kernel<T, false>), grid, dim3(NEAR_NT), 0, st, a, (int)per);
 }
 template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t st) {
     // V up to a multiple of 4 (8 above 32): the entries behind V cost arithmetic, and a row is never read past its end
