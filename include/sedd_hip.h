@@ -254,19 +254,18 @@ int sedd_post_norm_residual_fwd(const float* residual, const void* a, int a_dtyp
                                 sedd_stream_t stream);
 /* its backward: dx1 fp32 [M, D] = the gradient of x_out that does not come through y (NULL: zero; with dh only), dh (a_dtype,
  * or NULL: no norm behind) that of y.  d = dx1 + LayerNorm backward of dh;  dx = res_scale * d (dx may be dx1);  da (a_dtype) = the gradient of a.
- * ws fp32 [6, nchunk, D] ([3, nchunk, D] without dh), nchunk = sedd_post_norm_chunks(M, L, D): partial column sums, folded by
- * sedd_post_norm_residual_bwd_reduce into dgate [B, .] (row stride dgate_stride), dshift / dscale [B, .] (dmod_stride)
- * (written), and dpost_w, dbias (the column sums of da before its rounding: the bias gradient of the Linear that made a), dw
- * [D] (+=).  Any of them may be NULL.  Fixed order: bit-reproducible. */
+ * dgate [B, .] (row stride dgate_stride), dshift / dscale [B, .] (dmod_stride) are written; dpost_w, dbias (the column sums of
+ * da before its rounding: the bias gradient of the Linear that made a) and dw [D] are added to.  Any of the six may be NULL.
+ * ws fp32 [6, nchunk, D] ([3, nchunk, D] without dh), nchunk = sedd_post_norm_chunks(M, L, D): partial column sums, folded in a
+ * fixed order: bit-reproducible. */
 int sedd_post_norm_chunks(int64_t M, int64_t L, int D);
 int sedd_post_norm_residual_bwd(const float* dx1, const void* dh, const float* x1, const float* w, const void* scale,
                                 const float* mean, const float* rstd, const void* a, int a_dtype, const float* post_w,
                                 const void* gate, int mod_dtype, int64_t mod_stride, const float* post_mean,
                                 const float* post_rstd, float res_scale, float inv_keep, uint64_t seed, float p_drop,
-                                float* dx, void* da, float* ws, int64_t M, int64_t L, int D, sedd_stream_t stream);
-int sedd_post_norm_residual_bwd_reduce(const float* ws, float* dgate, int64_t dgate_stride, float* dshift, float* dscale,
-                                       int64_t dmod_stride, float* dpost_w, float* dbias, float* dw, int64_t M, int64_t L,
-                                       int D, sedd_stream_t stream);
+                                float* dx, void* da, float* dgate, int64_t dgate_stride, float* dshift, float* dscale,
+                                int64_t dmod_stride, float* dpost_w, float* dbias, float* dw, float* ws, int64_t M, int64_t L,
+                                int D, sedd_stream_t stream);
 
 /* Rotary (model/rotary.py:13-51): in-place NeoX rotation of the Q and K slots of qkv [B, L, 3, H, d]:
  * out = x*cos + rotate_half(x)*sin with rotate_half(x) = [-x2, x1]; conj != 0 applies the transposed rotation

@@ -49,8 +49,7 @@ SIGNATURES = {
     "sedd_gate_residual_ln_modulate_fwd": "ppipppil" + "flf" + "ppppp" + "llip",
     "sedd_post_norm_chunks": "lli",
     "sedd_post_norm_residual_fwd": "ppipppp" + "il" + "fflf" + "ppp" + "pppp" + "llip",
-    "sedd_post_norm_residual_bwd": "ppppppp" + "pipp" + "ilpp" + "fflf" + "ppp" + "llip",
-    "sedd_post_norm_residual_bwd_reduce": "pplppl" + "ppp" + "llip",
+    "sedd_post_norm_residual_bwd": "ppppppp" + "pipp" + "ilpp" + "fflf" + "pp" + "plppl" + "pppp" + "llip",
     "sedd_rotary_qkv": "pippiiiiip",
     "sedd_gelu_fwd": "ppilp",
     "sedd_gelu_bwd": "pppilp",

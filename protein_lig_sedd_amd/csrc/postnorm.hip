@@ -63,16 +63,17 @@ __global__ void __launch_bounds__(TPB) post_norm_fwd_kernel(
     }
     if (lane == 0) { pmean[row] = pm; prstd[row] = pr; }
     if constexpr (NEXT) {
-        const float mu = dpp_sum(s) * inv_d;
+        // in the steps of the plain LayerNorm kernel, so that h is to the bit what that makes of x1
+        const float mu = wave_sum(s) / (float)D;
         q = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (k * 256 + lane * 4 < D) {
-                v[k].x -= mu; v[k].y -= mu; v[k].z -= mu; v[k].w -= mu;
-                q += (v[k].x * v[k].x + v[k].y * v[k].y) + (v[k].z * v[k].z + v[k].w * v[k].w);
+                const float a = v[k].x - mu, b = v[k].y - mu, cc = v[k].z - mu, d = v[k].w - mu;
+                q += (a * a + b * b) + (cc * cc + d * d);
             }
         }
-        const float r1 = 1.0f / sqrtf(dpp_sum(q) * inv_d + 1e-5f);
+        const float r1 = 1.0f / sqrtf(wave_sum(q) / (float)D + 1e-5f);
         if (lane == 0) { mean[row] = mu; rstd[row] = r1; }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -80,10 +81,10 @@ __global__ void __launch_bounds__(TPB) post_norm_fwd_kernel(
             if (c < D) {
                 const float4 ww = load4<float>(w + c);
                 const float4 sc = load4<TM>(scale + b * mod_stride + c), sh = load4<TM>(shift + b * mod_stride + c);
-                store4<TA>(y + row * D + c, make_float4(v[k].x * r1 * ww.x * (1.f + sc.x) + sh.x,
-                                                        v[k].y * r1 * ww.y * (1.f + sc.y) + sh.y,
-                                                        v[k].z * r1 * ww.z * (1.f + sc.z) + sh.z,
-                                                        v[k].w * r1 * ww.w * (1.f + sc.w) + sh.w));
+                store4<TA>(y + row * D + c, make_float4((v[k].x - mu) * r1 * ww.x * (1.f + sc.x) + sh.x,
+                                                        (v[k].y - mu) * r1 * ww.y * (1.f + sc.y) + sh.y,
+                                                        (v[k].z - mu) * r1 * ww.z * (1.f + sc.z) + sh.z,
+                                                        (v[k].w - mu) * r1 * ww.w * (1.f + sc.w) + sh.w));
             }
         }
     }
@@ -150,11 +151,13 @@ extern "C" int sedd_post_norm_residual_fwd(const float* residual, const void* a,
 // da  = pr * (g2 - mean(g2) - ahat * mean(g2 ahat)),     g2 = dn * wp
 // dw += dh (1 + scale) xhat;  dshift = sum dh;  dscale = sum dh xhat w;  dgate = sum d keep ahat wp;  dwp += dn ahat;
 // dbias += da (before it is rounded: the bias gradient of the Linear that made a)
-// A block owns a chunk of rows of one batch element and a thread four columns of it, so the six column sums are running sums in
-// registers and leave as one line of partial sums per chunk: no fold across waves, which a wave-per-row layout needs for all
-// six.  What crosses the waves is two pairs of row sums, through LDS.  The next row's operands are loaded before this row's
-// sums are waited for.
-// Rows of a chunk (never across two batch elements): 32, or fewer where that leaves less than 2560 waves (10 a CU).  Measured with
+// A block owns a chunk of rows and a thread four columns of it, so the six column sums are running sums in registers and leave as
+// one line of partial sums per chunk: no fold across waves, which a wave-per-row layout needs for all six.  What crosses the
+// waves is two pairs of row sums, through LDS.  The next row's operands are loaded before this row's sums are waited for.
+// A chunk is a part of one batch element, a whole one where that is shorter than two chunks, or several where they are shorter
+// than half of one.  Where no batch element is split, the sums per batch element (dgate, dshift, dscale) are final and go straight
+// to their place (2703 x 4 x 1484: 112 us; with a chunk and a fold to each batch element 266 us).
+// Rows of a chunk: 32, or fewer where that leaves less than 2560 waves (10 a CU).  Measured with
 // half and twice the rows: 64 x 512 x 768 32 rows 113 us (16: 121, 64: 155); 16 x 1024 x 1024 16 rows 71 (8: 80, 32: 86);
 // 8 x 512 x 2048 8 rows 36 (4: 46); more waves cover the latency of the row sums, more chunks write more partial sums.
 static inline int post_chunk_rows(int64_t M, int D) {
@@ -163,10 +166,17 @@ static inline int post_chunk_rows(int64_t M, int D) {
     while (r > 4 && M / r * nw < 2560) r >>= 1;
     return r;
 }
-extern "C" int sedd_post_norm_chunks(int64_t M, int64_t L, int D) {
-    if (L <= 0 || M <= 0) return 0;
+struct PostChunks {
+    int64_t n, per_batch, batches;  // chunks; chunks of a batch element; batch elements of a chunk
+    int rows;                       // of a chunk at most
+};
+static PostChunks post_chunks(int64_t M, int64_t L, int D) {
     const int r = post_chunk_rows(M, D);
-    return (int)((M / L) * ((L + r - 1) / r));
+    const int64_t B = M / L, g = 2 * L <= r ? r / L : 1, per = L < 2 * r ? 1 : (L + r - 1) / r;
+    return {g > 1 ? (B + g - 1) / g : B * per, per, g, (int)(g > 1 ? g * L : (L + per - 1) / per)};
+}
+extern "C" int sedd_post_norm_chunks(int64_t M, int64_t L, int D) {
+    return L <= 0 || M <= 0 ? 0 : (int)post_chunks(M, L, D).n;
 }
 // both sums over the block's nw waves (buf: 2 nw floats; two buffers in turn: the next write to one comes after another barrier)
 __device__ __forceinline__ void block_sum2(float& a, float& b, float* buf, int nw) {
@@ -189,37 +199,69 @@ struct PostBwdArgs {
     const void *dh, *a, *scale, *gate;
     float *dx, *ws;
     void* da;
-    int64_t mod_stride, nchunk, L;
+    float* out[6];  // by plane: 0 dgate, 1 dwp, 2 dbias, 3 dw, 4 dshift, 5 dscale; any may be NULL
+    int64_t mod_stride, gate_stride, dmod_stride, L, B;
+    PostChunks ch;
     float alpha, inv_keep;
     uint64_t seed;
     uint32_t thr16;
-    int D, CR;
+    int D, planes;
 };
 template <typename TA, typename TM, bool NEXT>
 __global__ void __launch_bounds__(512) post_norm_bwd_kernel(PostBwdArgs p) {
     __shared__ float sA[2 * 8], sB[2][2 * 8];
     const int nw = blockDim.x >> 6, c = threadIdx.x * 4, D = p.D;
     const bool on = c < D;
-    const int64_t cpb = (p.L + p.CR - 1) / p.CR;
-    const int64_t chunk = blockIdx.x, b = chunk / cpb, c0 = (chunk % cpb) * p.CR;
-    const int nrows = (int)((p.L - c0) < p.CR ? (p.L - c0) : p.CR);
+    const int64_t chunk = blockIdx.x;
+    int64_t b = p.ch.batches > 1 ? chunk * p.ch.batches : chunk / p.ch.per_batch;
+    const int64_t row0 = p.ch.batches > 1 ? b * p.L : b * p.L + chunk % p.ch.per_batch * p.ch.rows;
+    const int64_t left = (p.ch.batches > 1 ? p.B * p.L : (b + 1) * p.L) - row0;
+    const int nrows = left < p.ch.rows ? (int)left : p.ch.rows;
+    int batch_end = p.ch.batches > 1 ? (int)p.L : nrows;  // the row behind the batch element at hand
     const float inv_d = 1.0f / (float)D;
     uint64_t seed = p.seed;
     if (p.thr16) seed = resolve_seed(seed);
     const TA *dh = (const TA*)p.dh, *a = (const TA*)p.a;
     TA* da = (TA*)p.da;
     float4 wp = f4(0.f), gt = f4(0.f), ww = f4(0.f), sc1 = f4(0.f);
-    if (on) {
-        wp = load4<float>(p.wp + c);
+    auto modulation = [&]() __attribute__((always_inline)) {
+        if (!on) return;
         gt = load4<TM>((const TM*)p.gate + b * p.mod_stride + c);
         if constexpr (NEXT) {
-            ww = load4<float>(p.w + c);
             const float4 s = load4<TM>((const TM*)p.scale + b * p.mod_stride + c);
             sc1 = make_float4(1.f + s.x, 1.f + s.y, 1.f + s.z, 1.f + s.w);
         }
+    };
+    if (on) {
+        wp = load4<float>(p.wp + c);
+        if constexpr (NEXT) ww = load4<float>(p.w + c);
     }
+    modulation();
     float4 aw = f4(0.f), ash = f4(0.f), asc = f4(0.f), ag = f4(0.f), apw = f4(0.f), ab = f4(0.f);
-    const int64_t row0 = b * p.L + c0;
+    // the sums of a batch element: final, or a line of partial sums
+    auto flush = [&]() __attribute__((always_inline)) {
+        if (!on) return;
+        if (p.ch.per_batch == 1) {
+            auto put = [&](float* o, int64_t stride, const float4& v) {  // (scalar: a gradient slice need not be 16-byte aligned)
+                if (!o) return;
+                o += b * stride + c;
+                o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+            };
+            put(p.out[0], p.gate_stride, ag);
+            if constexpr (NEXT) {
+                put(p.out[4], p.dmod_stride, ash);
+                put(p.out[5], p.dmod_stride, asc);
+            }
+        } else {
+            float* o = p.ws + chunk * D + c;
+            const int64_t plane = p.ch.n * D;
+            store4<float>(o, ag);
+            if constexpr (NEXT) {
+                store4<float>(o + 4 * plane, ash);
+                store4<float>(o + 5 * plane, asc);
+            }
+        }
+    };
     float4 dn = f4(0.f), an = f4(0.f), gn = f4(0.f), xn = f4(0.f);  // the next row
     auto fetch = [&](int i) __attribute__((always_inline)) {
         if (!on) return;
@@ -294,46 +336,61 @@ __global__ void __launch_bounds__(512) post_norm_bwd_kernel(PostBwdArgs p) {
             }
             store4<TA>(da + off, o);
         }
+        if (i + 1 == batch_end && i + 1 < nrows) {
+            flush();
+            ag = ash = asc = f4(0.f);
+            batch_end += (int)p.L;
+            ++b;
+            modulation();
+        }
     }
+    flush();
     if (on) {
         float* o = p.ws + chunk * D + c;
-        const int64_t plane = p.nchunk * D;
-        store4<float>(o, ag);
+        const int64_t plane = p.ch.n * D;
         store4<float>(o + plane, apw);
         store4<float>(o + 2 * plane, ab);
-        if constexpr (NEXT) {
-            store4<float>(o + 3 * plane, aw);
-            store4<float>(o + 4 * plane, ash);
-            store4<float>(o + 5 * plane, asc);
-        }
+        if constexpr (NEXT) store4<float>(o + 3 * plane, aw);
     }
 }
 
-// Folds the chunk partials in a fixed order.  Planes: 0 dgate, 1 dwp, 2 dbias, 3 dw, 4 dshift, 5 dscale; 0, 4 and 5 are sums
-// per batch element (written), 1, 2 and 3 over all chunks (added to what is there).  Any output may be NULL.  A block folds 64
-// columns: 16 lanes of four columns each, 16 groups of lines that meet in LDS.  The few long folds come first, with 8 loads in
-// flight per thread: they are bound by latency.
-struct PostReduceArgs {
-    const float* ws;
-    float* out[6];
-    int64_t gate_stride, mod_stride, nchunk, cpb, B;
-    int D, np;
-};
-__global__ void __launch_bounds__(TPB) post_norm_reduce_kernel(PostReduceArgs p) {
-    const int ncb = (p.D + 63) / 64, nvec = p.np == 6 ? 3 : 2;
+// Folds the chunks' partial sums in a fixed order: planes 1, 2 and 3 over all chunks (added to what is there) and, where batch
+// elements are split, 0, 4 and 5 over each one's (written).  A block folds 64 columns: 16 lanes of four columns each, 16 groups
+// of lines that meet in LDS, or, where a batch element has fewer lines than that, 16 batch elements.  The few long folds come
+// first, with 8 loads in flight per thread: they are bound by latency.
+__host__ __device__ __forceinline__ int64_t fold_batches(const PostChunks& ch) { return ch.per_batch < 16 ? 16 : 1; }
+__global__ void __launch_bounds__(TPB) post_norm_reduce_kernel(PostBwdArgs p) {
+    const int ncb = (p.D + 63) / 64, nvec = p.planes == 6 ? 3 : 2;
+    const int64_t fb = fold_batches(p.ch), nb = (p.B + fb - 1) / fb;
     const bool vec = (int64_t)blockIdx.x < (int64_t)nvec * ncb;
     int64_t i = vec ? blockIdx.x : blockIdx.x - (int64_t)nvec * ncb;
     const int col = (int)(i % ncb) * 64 + (threadIdx.x & 15) * 4, rg = threadIdx.x >> 4;
     i /= ncb;
-    const int64_t b = vec ? 0 : i % p.B;
-    const int k = vec ? 1 + (int)i : (i / p.B == 0 ? 0 : 3 + (int)(i / p.B));
+    const int64_t b = vec ? 0 : i % nb * fb + (fb > 1 ? rg : 0);
+    const int k = vec ? 1 + (int)i : (i / nb == 0 ? 0 : 3 + (int)(i / nb));
     float* out = p.out[k];
     if (!out) return;
+    auto put = [&](const float4& v) {  // (scalar accesses: a gradient slice need not be 16-byte aligned)
+        float* o = out + b * (k == 0 ? p.gate_stride : p.dmod_stride) + col;
+        o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+    };
+    if (!vec && fb > 1) {
+        if (col >= p.D || b >= p.B) return;
+        const float* base = p.ws + ((int64_t)k * p.ch.n + b * p.ch.per_batch) * p.D + col;
+        float4 s = f4(0.f);
+#pragma unroll 8
+        for (int64_t c = 0; c < p.ch.per_batch; ++c) {
+            const float4 v = load4<float>(base + c * p.D);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        put(s);
+        return;
+    }
     __shared__ float4 red[16][16];
-    const int64_t lines = vec ? p.nchunk : p.cpb;
+    const int64_t lines = vec ? p.ch.n : p.ch.per_batch;
     float4 s = f4(0.f);
     if (col < p.D) {
-        const float* base = p.ws + ((int64_t)k * p.nchunk + b * p.cpb) * p.D + col;
+        const float* base = p.ws + ((int64_t)k * p.ch.n + b * p.ch.per_batch) * p.D + col;
         int64_t c = rg;
         for (; c + 7 * 16 < lines; c += 8 * 16) {
             float4 v[8];
@@ -354,12 +411,8 @@ __global__ void __launch_bounds__(TPB) post_norm_reduce_kernel(PostReduceArgs p)
             const float4 v = red[r][threadIdx.x];
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
-        // (scalar accesses: a gradient slice need not be 16-byte aligned)
         if (vec) { out[col] += s.x; out[col + 1] += s.y; out[col + 2] += s.z; out[col + 3] += s.w; }
-        else {
-            float* o = out + b * (k == 0 ? p.gate_stride : p.mod_stride) + col;
-            o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
-        }
+        else put(s);
     }
 }
 
@@ -368,7 +421,9 @@ extern "C" int sedd_post_norm_residual_bwd(const float* dx1, const void* dh, con
                                            int a_dtype, const float* post_w, const void* gate, int mod_dtype,
                                            int64_t mod_stride, const float* post_mean, const float* post_rstd,
                                            float res_scale, float inv_keep, uint64_t seed, float p_drop, float* dx,
-                                           void* da, float* ws, int64_t M, int64_t L, int D, sedd_stream_t stream) {
+                                           void* da, float* dgate, int64_t dgate_stride, float* dshift, float* dscale,
+                                           int64_t dmod_stride, float* dpost_w, float* dbias, float* dw, float* ws,
+                                           int64_t M, int64_t L, int D, sedd_stream_t stream) {
     int rc = post_norm_check("post_norm_residual_bwd", a_dtype, mod_dtype, mod_stride, p_drop, M, L, D);
     if (rc) return rc;
     if (M == 0) return SEDD_OK;
@@ -382,31 +437,19 @@ extern "C" int sedd_post_norm_residual_bwd(const float* dx1, const void* dh, con
     PostBwdArgs p;
     p.dx1 = dx1; p.x1 = x1; p.w = w; p.mean = mean; p.rstd = rstd; p.wp = post_w; p.pmean = post_mean; p.prstd = post_rstd;
     p.dh = dh; p.a = a; p.scale = scale; p.gate = gate; p.dx = dx; p.ws = ws; p.da = da;
-    p.mod_stride = mod_stride; p.nchunk = sedd_post_norm_chunks(M, L, D); p.L = L; p.alpha = res_scale; p.inv_keep = inv_keep;
-    p.seed = seed; p.thr16 = (uint32_t)(p_drop * 65536.0f + 0.5f); p.D = D; p.CR = post_chunk_rows(M, D);
-    const dim3 grid((unsigned)p.nchunk), block((unsigned)((D + 255) / 256 * 64));
+    float* outs[6] = {dgate, dpost_w, dbias, dw, dshift, dscale};
+    for (int k = 0; k < 6; ++k) p.out[k] = outs[k];
+    p.mod_stride = mod_stride; p.gate_stride = dgate_stride; p.dmod_stride = dmod_stride; p.L = L; p.B = M / L;
+    p.ch = post_chunks(M, L, D); p.alpha = res_scale; p.inv_keep = inv_keep;
+    p.seed = seed; p.thr16 = (uint32_t)(p_drop * 65536.0f + 0.5f); p.D = D; p.planes = dh ? 6 : 3;
+    const dim3 grid((unsigned)p.ch.n), block((unsigned)((D + 255) / 256 * 64));
     DISPATCH_DT(a_dtype, TA, DISPATCH_DT(mod_dtype, TM, {
         if (dh) hipLaunchKernelGGL((post_norm_bwd_kernel<TA, TM, true>), grid, block, 0, (hipStream_t)stream, p);
         else hipLaunchKernelGGL((post_norm_bwd_kernel<TA, TM, false>), grid, block, 0, (hipStream_t)stream, p);
     }));
-    SEDD_LAUNCH_CHECK();
-    return SEDD_OK;
-}
-
-extern "C" int sedd_post_norm_residual_bwd_reduce(const float* ws, float* dgate, int64_t dgate_stride, float* dshift,
-                                                  float* dscale, int64_t dmod_stride, float* dpost_w, float* dbias,
-                                                  float* dw, int64_t M, int64_t L, int D, sedd_stream_t stream) {
-    SEDD_CHECK_ARG(M >= 0 && L > 0 && M % L == 0 && D > 0 && D % 4 == 0, "post_norm_residual_bwd_reduce: bad sizes");
-    if (M == 0) return SEDD_OK;
-    SEDD_CHECK_ARG(ws, "post_norm_residual_bwd_reduce: ws is null");
-    PostReduceArgs p;
-    p.ws = ws;
-    float* outs[6] = {dgate, dpost_w, dbias, dw, dshift, dscale};
-    for (int k = 0; k < 6; ++k) p.out[k] = outs[k];
-    p.gate_stride = dgate_stride; p.mod_stride = dmod_stride; p.nchunk = sedd_post_norm_chunks(M, L, D); p.B = M / L; p.cpb = p.nchunk / p.B; p.D = D;
-    p.np = (dw || dshift || dscale) ? 6 : 3;
-    const int64_t blocks = (int64_t)((D + 63) / 64) * (p.np == 6 ? 3 + 3 * p.B : 2 + p.B);
-    hipLaunchKernelGGL(post_norm_reduce_kernel, dim3((unsigned)blocks), dim3(TPB), 0, (hipStream_t)stream, p);
+    const int64_t fb = fold_batches(p.ch), nb = (p.B + fb - 1) / fb;
+    const int64_t folds = (p.planes == 6 ? 3 : 2) + (p.ch.per_batch > 1 ? (p.planes == 6 ? 3 : 1) * nb : 0);
+    hipLaunchKernelGGL(post_norm_reduce_kernel, dim3((unsigned)((D + 63) / 64 * folds)), dim3(TPB), 0, (hipStream_t)stream, p);
     SEDD_LAUNCH_CHECK();
     return SEDD_OK;
 }

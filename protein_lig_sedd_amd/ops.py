@@ -854,11 +854,9 @@ def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=Non
                                                               + (0 if norm is None else 4 + a.element_size()))):
             check(lib().sedd_post_norm_residual_bwd(_p(dx1), _p(dh), _p(x1), _p(w), _p(scale), _p(mean), _p(rstd), _p(a), _dt(a),
                                                     _p(post_w), _p(gate), _dt(gate), ms, _p(pm), _p(pr), float(res_scale),
-                                                    float(inv_keep), seed, pd, _p(dx), _p(da), _p(ws), M, L, D, _stream()),
-                  "sedd_post_norm_residual_bwd")
-            check(lib().sedd_post_norm_residual_bwd_reduce(_p(ws), _p(dgate), gs, _p(dshift), _p(dscale), dms, _p(dpost_w),
-                                                           _p(dbias), _p(dw), M, L, D, _stream()),
-                  "sedd_post_norm_residual_bwd_reduce")
+                                                    float(inv_keep), seed, pd, _p(dx), _p(da), _p(dgate), gs, _p(dshift),
+                                                    _p(dscale), dms, _p(dpost_w), _p(dbias), _p(dw), _p(ws), M, L, D,
+                                                    _stream()), "sedd_post_norm_residual_bwd")
     return dx, da
 
 

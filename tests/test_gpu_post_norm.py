@@ -150,10 +150,28 @@ def test_widths(D, dtype):
 
 @pytest.mark.parametrize("B,L", [(1, 1), (1, 2), (7, 1), (1, 31), (2, 32), (2, 33), (3, 65), (1, 400), (40, 420)])
 def test_lengths(B, L):
-    """chunks of 32 rows (64 from 16384 rows up), whole and cut off"""
+    """chunks of 4 to 32 rows, whole and cut off"""
     check(B, L, 64, torch.bfloat16, True, 1.0)
     check(B, L, 64, torch.float32, False, 0.5)
     check(B, L, 64, torch.float32, True, 1.0, dx1=False)
+
+
+@pytest.mark.parametrize("B,L,D", [(11, 1, 1028), (9, 2, 96), (5, 3, 64), (30001, 1, 32), (16003, 3, 32), (16000, 2, 100)])
+def test_short_batch_elements(B, L, D):
+    """several whole batch elements to a chunk, the last chunk not full; 5 x 3: one to a chunk"""
+    check(B, L, D, torch.bfloat16, True, 1.0)
+    check(B, L, D, torch.float32, False, 0.5)
+
+
+@pytest.mark.parametrize("D", [36, 256, 516, 768, 1024, 1484, 2048])
+def test_next_norm_is_the_plain_norm_to_the_bit(D):
+    """blocks that are joined at their boundary and blocks that are not give the same activations"""
+    from protein_lig_sedd_amd import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        s = make(4, 300, D, dtype)
+        x1, h, (_, _, mean, rstd) = run_fwd(s, 0.9, True)
+        y, m, r = ops.ln_modulate_fwd(x1, s["w"], s["shift"], s["scale"], out_dtype=dtype)
+        assert torch.equal(h.view(-1), y.view(-1)) and torch.equal(mean, m.view(-1)) and torch.equal(rstd, r.view(-1))
 
 
 def test_types_of_activations_and_modulation():

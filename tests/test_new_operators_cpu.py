@@ -39,9 +39,10 @@ def _fwd(L, p, a_dtype=0, mod_dtype=0, stride=64, p_drop=0.0, w=None, nxt=None, 
                                          nxt, nxt, M, Ln, D, None)
 
 
-def _bwd(L, p, dh=None, a_dtype=0, mod_dtype=0, stride=64, p_drop=0.0, M=4, Ln=2, D=64, dx1=0, x1=None):
+def _bwd(L, p, dh=None, a_dtype=0, mod_dtype=0, stride=64, p_drop=0.0, M=4, Ln=2, D=64, dx1=0, x1=None, ws=0):
     return L.sedd_post_norm_residual_bwd(p if dx1 == 0 else dx1, dh, x1, x1, x1, x1, x1, p, a_dtype, p, p, mod_dtype, stride, p, p,
-                                         1.0, 1.0, 0, p_drop, p, p, p, M, Ln, D, None)
+                                         1.0, 1.0, 0, p_drop, p, p, p, 64, None, None, 64, None, None, None,
+                                         p if ws == 0 else ws, M, Ln, D, None)
 
 
 def test_post_norm_refusals(ptr):
@@ -56,8 +57,10 @@ def test_post_norm_refusals(ptr):
         assert fn(L, None, M=0) == 0
     assert _fwd(L, ptr, w=ptr) == -1 and _bwd(L, ptr, dh=ptr) == -1  # a next norm without its tensors
     assert _bwd(L, ptr, dx1=None) == -1                              # neither gradient
-    assert L.sedd_post_norm_residual_bwd_reduce(None, None, 64, None, None, 64, None, None, None, 4, 2, 64, None) == -1
-    assert L.sedd_post_norm_residual_bwd_reduce(None, None, 64, None, None, 64, None, None, None, 0, 2, 64, None) == 0
+    assert _bwd(L, ptr, ws=None) == -1
+    assert L.sedd_post_norm_chunks(0, 4, 64) == 0 and L.sedd_post_norm_chunks(4, 0, 64) == 0
+    assert L.sedd_post_norm_chunks(64 * 1024, 1024, 768) == 64 * 32  # parts of a batch element
+    assert L.sedd_post_norm_chunks(64 * 1024, 4, 768) == 64 * 32     # several to a chunk
 
 
 def test_multi_tensor_refusals(ptr):
