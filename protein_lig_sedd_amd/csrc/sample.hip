@@ -997,15 +997,23 @@ template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t
     else if (a.V <= 40) launch_lane<T, 40>(a, st);
     else if (a.V <= 48) launch_lane<T, 48>(a, st);
     else if (a.V <= 64) launch_lane<T, 64>(a, st);
-    // a wave per row while its entries fit 64 a lane, four waves up to 16384, sixteen up to 32768 (32 a lane: such a block has
-    // 128 registers a lane)
+    // A wave per row up to 3000 entries, four waves up to 16384, sixteen up to 32768 (32 a lane: such a block has 128 registers
+    // a lane).  Few rows leave most of the card idle and a pass over a row is what a call waits for: then four times the waves.
+    // us, bf16, with top-p 0.3 | top-k 500 and top-p 0.3, one wave / four waves (V = 12000: four / sixteen):
+    //   V =  2365:    64 rows 24 / 19 | 36 / 23;  512 rows 33 / 24 | 47 / 47;  2048 rows 46 / 43 | 59 / 85
+    //   V =  3900:    64 rows 46 / 20 | 58 / 26;  512 rows 69 / 27 | 86 / 31;  8192 rows 188 / 105 | 248 / 196
+    //   V = 12000:    64 rows 61 / 38 | 76 / 45;  256 rows 60 / 38 | 95 / 52;  2048 rows 218 / 174 | 274 / 405
+    // (V = 600: no difference up to 512 rows.)
+    else if (a.V > 1024 && a.V <= 2048 && a.M <= 512) launch_wide<T, 4, 8>(a, st);
+    else if (a.V > 2048 && a.V <= 4096 && (a.M <= 512 || a.V > 3000)) launch_wide<T, 4, 16>(a, st);
+    else if (a.V > 4096 && a.V <= 8192 && a.M <= 256) launch_wide<T, 16, 8>(a, st);
+    else if (a.V > 8192 && a.V <= 16384 && a.M <= 256) launch_wide<T, 16, 16>(a, st);
     else if (a.V <= 256) launch_wide<T, 1, 4>(a, st);
     else if (a.V <= 512) launch_wide<T, 1, 8>(a, st);
     else if (a.V <= 1024) launch_wide<T, 1, 16>(a, st);
     else if (a.V <= 2048) launch_wide<T, 1, 32>(a, st);
     else if (a.V <= 2560) launch_wide<T, 1, 40>(a, st);
-    else if (a.V <= 48 * 64) launch_wide<T, 1, 48>(a, st);
-    else if (a.V <= 4096) launch_wide<T, 1, 64>(a, st);
+    else if (a.V <= 3000) launch_wide<T, 1, 48>(a, st);
     else if (a.V <= 8192) launch_wide<T, 4, 32>(a, st);
     else if (a.V <= 16384) launch_wide<T, 4, 64>(a, st);
     else if (a.V <= 32768) launch_wide<T, 16, 32>(a, st);

@@ -86,6 +86,22 @@ def test_wide_vocabularies(V, rows, dtype):
         check(x, u, **c)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,rows", [(1025, 600), (2047, 600), (2365, 513), (2600, 600), (3000, 600), (3001, 600), (4097, 300), (8200, 260),
+                                    (12001, 257), (16384, 257)])
+def test_wide_vocabularies_in_many_rows(V, rows, dtype):
+    """what many rows decide is what the formulas say of some of them, and what few rows at a time decide of all"""
+    from protein_lig_sedd_amd import ops
+    x, u = data((rows, V), dtype, V)
+    some = [0, 1, rows // 2, rows - 1]
+    for c in CUTS + [dict(top_k=V // 2, top_p=0.5)]:
+        got = ops.sample_truncated(x, u, **c)
+        want = ref(x[some], u[some], c.get("temperature", 1.0), c.get("top_k", 0), c.get("top_p", 1.0), c.get("min_p", 0.0))
+        assert torch.equal(got[some].cpu(), want), c
+        parts = [ops.sample_truncated(x[i:i + 100], u[i:i + 100], **c) for i in range(0, rows, 100)]
+        assert torch.equal(got, torch.cat(parts)), c
+
+
 @pytest.mark.parametrize("V", [26, 64, 300, 5000])
 def test_many_rows_and_one(V):
     for rows in (1, 255, 256, 257, 2000 if V < 1000 else 40):
