@@ -54,8 +54,7 @@ __device__ __forceinline__ float gelu_tanh_grad_f(float u) {
     const float t = tanhf(0.7978845608028654f * (u + 0.044715f * u * u * u));
     return 0.5f * (1.0f + t) + 0.5f * u * (1.0f - t * t) * 0.7978845608028654f * (1.0f + 3.0f * 0.044715f * u * u);
 }
-// Four elements at a time in the bf16 epilogues, written on ext-vector types so the polynomial parts compile to packed
-// fp32 ops (v_pk_mul/fma/add_f32, two elements per instruction): with s = sigmoid(2a) = 1 / (1 + 2^(u (A + B u^2))),
+// Four elements at a time in the bf16 epilogues: with s = sigmoid(2a) = 1 / (1 + 2^(u (A + B u^2))),
 // gelu_tanh(u) = u s and gelu_tanh'(u) = s (1 + u (1 - s)(C + D u^2)) — 5 resp. 9 plain operations + exp2 + rcp per
 // element instead of ~12 / ~22 through tanh (the fused dGELU epilogue is VALU-bound: every wave of the block is in it at
 // the same time, nothing overlaps it).  fp32 outputs keep the exact tanhf forms.
@@ -808,7 +807,10 @@ gemm_bf16_big_kernel(const bf16_t* __restrict__ A, int64_t lda,
                     // multiplier tile straight from global memory in the accumulator layout (lane: row lane & 15, the 4
                     // columns of fragment n): 8-byte loads, the four fragments of a row together cover its 128-byte line;
                     // no LDS round trip and no sigmoid — the pass is a multiply, the column sums and the store
-                    constexpr int PD = TM;  // every pass in flight at once: the fragment registers are free here
+                    // Two passes in flight.  What a pass leaves is pinned (the empty asm): without packed fp32 the compiler
+                    // otherwise holds products and sums of several passes, and the 256-row tile spills 408 bytes a lane
+                    // (D 768, 64 x 512 tokens: 358 us a launch; pinned, two passes in flight, 20 bytes: 237 us)
+                    constexpr int PD = TM < 2 ? TM : 2;
                     uint2 mv[PD][4];
 #define DMUL_LOAD(pass_)                                                                                             \
     _Pragma("unroll") for (int n = 0; n < 4; ++n) {                                                                  \
@@ -825,13 +827,17 @@ gemm_bf16_big_kernel(const bf16_t* __restrict__ A, int64_t lda,
                             union { uint2 u; TO e[4]; } pv;
                             pv.u = mv[pass % PD][n];
                             f32x4& v = acc[pass][n];
+                            float w[4], c[4];
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 // the reference rounds the Linear's data gradient to the activation dtype before GELU's
                                 const float dy = to_f32<TO>(from_f32<TO>(v[r]));
-                                v[r] = to_f32<TO>(from_f32<TO>(dy * to_f32<TO>(pv.e[r])));
-                                cs[n][r] += v[r];  // (rows / columns beyond the matrix: multiplier 0, so they add 0)
+                                w[r] = to_f32<TO>(from_f32<TO>(dy * to_f32<TO>(pv.e[r])));
+                                c[r] = cs[n][r] + w[r];  // (rows / columns beyond the matrix: multiplier 0, so they add 0)
                             }
+                            asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3]));
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) { v[r] = w[r]; cs[n][r] = c[r]; }
                         }
                         if (pass + PD < TM) DMUL_LOAD(pass + PD)
 #pragma unroll
@@ -867,13 +873,17 @@ gemm_bf16_big_kernel(const bf16_t* __restrict__ A, int64_t lda,
                         f32x4& v = acc[pass][n];
                         const f32x4 gp = gelu_grad4_t<TO>((f32x4){to_f32<TO>(pv.e[0]), to_f32<TO>(pv.e[1]),
                                                                   to_f32<TO>(pv.e[2]), to_f32<TO>(pv.e[3])});
+                        float w[4], c[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             // the reference rounds the Linear's data gradient to the activation dtype before GELU's
                             const float dy = to_f32<TO>(from_f32<TO>(v[r]));
-                            v[r] = to_f32<TO>(from_f32<TO>(dy * gp[r]));
-                            cs[n][r] += rok ? v[r] : 0.f;
+                            w[r] = to_f32<TO>(from_f32<TO>(dy * gp[r]));
+                            c[r] = cs[n][r] + (rok ? w[r] : 0.f);
                         }
+                        asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]), "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3]));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) { v[r] = w[r]; cs[n][r] = c[r]; }
                     }
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
