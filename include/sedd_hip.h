@@ -101,7 +101,7 @@ int sedd_philox_uniform(uint64_t seed, uint64_t offset, float* u, int64_t M, int
  * x (int64 [M], may be NULL): current tokens — only rows that hold mask_id are sampled, the others keep theirs, and a row with
  * nothing to sample keeps mask_id.  move (fp32 per batch element, with x only, may be NULL): a masked row is sampled only
  * where u[r][V] < move[r / L] (ldu >= V + 1 then): the ancestral update of an absorbing graph whose mask column is V.
- * HBM bytes M (V (e + 4) + 8) over the sampled rows. */
+ * out may not be x.  Fewer than 2^26 rows (2^32 for V <= 64).  HBM bytes M (V (e + 4) + 8) over the sampled rows. */
 int sedd_sample_truncated(const void* logits, int dtype, int64_t ld, const float* u, int64_t ldu, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, float temperature0, int top_k0,
                           float top_p0, float min_p0, const int64_t* x, int64_t mask_id, const float* move, int64_t* out,
@@ -246,7 +246,7 @@ int sedd_gate_residual_ln_modulate_fwd(const float* residual, const void* a, int
  *   n = LN(a) * post_w;  x_out = res_scale * residual + gate_b * dropout(n);  y = LN(x_out) * w * (1 + scale_b) + shift_b
  * residual / x_out fp32 [M, D]; a / y in a_dtype; gate / shift / scale rows of mod_dtype with row stride mod_stride;
  * post_mean / post_rstd / mean / rstd fp32 [M] saved for backward.  w == NULL: no norm behind it (shift, scale, y, mean, rstd
- * are not used).  Dropout by the (seed, p_drop) hash.  D % 4 == 0, D <= 2048. */
+ * are not used).  Dropout by the (seed, p_drop) hash.  D % 4 == 0, D <= 2048, M < 2^26. */
 int sedd_post_norm_residual_fwd(const float* residual, const void* a, int a_dtype, const float* post_w, const void* gate,
                                 const void* shift, const void* scale, int mod_dtype, int64_t mod_stride, float res_scale,
                                 float inv_keep, uint64_t seed, float p_drop, const float* w, float* x_out, void* y,

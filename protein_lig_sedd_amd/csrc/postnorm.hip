@@ -101,6 +101,7 @@ static int post_norm_check(const char* nm, int a_dtype, int mod_dtype, int64_t m
     SEDD_CHECK_ARG(dt_ok(a_dtype) && dt_ok(mod_dtype), "%s: bad dtype", nm);
     SEDD_CHECK_ARG(p_drop >= 0.f && p_drop < 1.f, "%s: p_drop %f", nm, (double)p_drop);
     SEDD_CHECK_ARG(M >= 0 && L > 0 && M % L == 0, "%s: bad sizes M=%ld L=%ld", nm, (long)M, (long)L);
+    SEDD_CHECK_ARG(M <= ((int64_t)1 << 26) - 4, "%s: %ld rows", nm, (long)M);  // (a wave each, 2^32 - 1 threads to a launch)
     if (D <= 0 || D % 4 != 0 || D > 2048 || mod_stride % 4 != 0) {
         sedd_set_error("%s: D=%d unsupported (need D %% 4 == 0, D <= 2048)", nm, D);
         return SEDD_ERR_UNSUPPORTED_SHAPE;

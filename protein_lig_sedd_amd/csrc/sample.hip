@@ -1028,6 +1028,9 @@ extern "C" int sedd_sample_truncated(const void* logits, int dtype, int64_t ld, 
     SEDD_CHECK_ARG(dtype == SEDD_F32 || dtype == SEDD_BF16, "sample_truncated: unknown dtype %d", dtype);
     SEDD_CHECK_ARG(M >= 0 && L > 0 && V > 0 && M % L == 0, "sample_truncated: bad sizes M=%ld L=%ld V=%d", (long)M,
                    (long)L, V);
+    // (a launch has at most 2^32 - 1 threads: 256 to four rows, or to one above 3000 entries, where memory ends before)
+    SEDD_CHECK_ARG(M <= ((int64_t)1 << 26) - 4 || (V <= 64 && M <= ((int64_t)1 << 32) - 256), "sample_truncated: %ld rows of %d entries",
+                   (long)M, V);
     SEDD_CHECK_ARG(M <= 1 || (ld >= V && ldu >= V + (move ? 1 : 0)), "sample_truncated: row strides %ld, %ld below V=%d",
                    (long)ld, (long)ldu, V);
     SEDD_CHECK_ARG(!move || x, "sample_truncated: move probabilities without current tokens");
@@ -1038,6 +1041,7 @@ extern "C" int sedd_sample_truncated(const void* logits, int dtype, int64_t ld, 
     SEDD_CHECK_ARG(top_k || top_k0 >= 0, "sample_truncated: top_k %d is negative", top_k0);
     if (M == 0) return SEDD_OK;
     SEDD_CHECK_ARG(logits && u && out, "sample_truncated: null pointer");
+    SEDD_CHECK_ARG(out != x, "sample_truncated: out is x");  // (a row that came near is looked at again after out was written)
     const SampleArgs a{logits, ld, u, ldu, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0,
                        x, mask_id, move, out, M, L, V};
     if (dtype == SEDD_F32) launch_sample<float>(a, (hipStream_t)stream);

@@ -116,6 +116,8 @@ class DualTrackDiffusionTransformer(nn.Module):
     def __init__(self, config, vocab_size_protein, vocab_size_ligand, compute_dtype=torch.float32,
                  seq_axis_attention=False):
         super().__init__()
+        if _cfg(config, "model.post_norm", False) or _cfg(config, "model.residual_scale", 1.0) not in (None, 1.0):
+            raise ValueError("the dual-track model has no post_norm / residual_scale")
         self.config = config
         self.enable_cross_attention = _cfg(config, "model.enable_cross_attention", True)
         hidden, cond, heads = _cfg(config, "model.hidden_size"), _cfg(config, "model.cond_dim"), _cfg(config, "model.n_heads")

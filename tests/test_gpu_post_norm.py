@@ -9,6 +9,7 @@ lose as much again: norm-wise 96 x 2^-24 forward, twice that backward, whose mea
 one likes: with |f - f'| <= e (|f| + rms f) for both factors of a product, the product is off by at most
 2 e (|f| + rms f)(|g| + rms g).  So a column sum of n products is off by (2 x 96 + n) x 2^-24 of the sum of those sizes: n for its
 adds.  bf16 results add half a step, 2^-8 of the value."""
+import math
 import types
 
 import pytest
@@ -443,6 +444,36 @@ def test_bf16_chained_equals_unchained(monkeypatch):
     for n, v in got[0][1].items():
         # (sums in another order: fp32 roundings of bf16 gradients, half a bf16 step where one of them flips)
         assert float((v - got[1][1][n]).norm()) <= 2.0 ** -8 * float(v.norm()) + 1e-12, n
+
+
+@pytest.mark.parametrize("cdt", [torch.float32, torch.bfloat16])
+def test_trainer_eager_captured_and_with_a_second_stream(cdt):
+    """the trainer's fused step on a post-norm model: one captured step replayed, and weight gradients on a second stream, leave
+    the bits of the eager steps"""
+    from protein_lig_sedd_amd import graph_lib, noise_lib
+    from protein_lig_sedd_amd.model.transformer import _SEDD
+    from protein_lig_sedd_amd.train import SEDDTrainer
+    B, L, steps = 4, 48, 6
+    graph, noise = graph_lib.Absorbing(25), noise_lib.LogLinearNoise(eps=1e-3).to(DEV)
+    g = torch.Generator().manual_seed(9)
+    xs = [torch.randint(0, 25, (B, L), generator=g).to(DEV) for _ in range(steps)]
+    ts = [(torch.rand(B, generator=g) * 0.9 + 0.05).to(DEV) for _ in range(steps)]
+    us = [torch.rand(B, L, generator=g).to(DEV) for _ in range(steps)]
+
+    def run(**kw):
+        model = seeded(_SEDD(config(D=128, blocks=2), compute_dtype=cdt)).to(DEV)
+        tr = SEDDTrainer(model, noise, graph, dict(lr=1e-3, warmup=3, grad_clip=1.0, weight_decay=0.01), world_size=1, **kw)
+        losses = [float(tr.train_step(xs[i], t=ts[i], u=us[i])) for i in range(steps)]
+        torch.cuda.synchronize()
+        return losses, tr
+
+    eager, te = run()
+    assert eager[-1] != eager[0] and all(map(math.isfinite, eager))
+    for kw in (dict(hip_graph=True), dict(wgrad_stream=True)):
+        losses, tr = run(**kw)
+        assert losses == eager, kw
+        for name in ("p", "m", "v", "ema"):
+            assert torch.equal(getattr(tr.flat, name), getattr(te.flat, name)), (kw, name)
 
 
 # ------------------------------------------------------------------------------------- the three operators together

@@ -27,11 +27,14 @@ def test_sample_truncated_refusals(ptr):
     L = _lib()
     for kw in (dict(dtype=7), dict(M=5), dict(Ln=0), dict(V=0), dict(M=-1), dict(ld=25), dict(ldu=25), dict(T=-1.0),
                dict(T=math.nan), dict(T=math.inf), dict(P=1.5), dict(P=math.nan), dict(m=-0.5), dict(k=-2), dict(move=ptr),
-               dict(x=ptr, move=ptr)):  # (the last: no column for the move numbers)
+               dict(x=ptr, move=ptr), dict(x=ptr)):  # (the last two: no column for the move numbers; out is x)
         assert _sample(L, ptr, **kw) == -1, kw
         assert b"sample_truncated" in L.sedd_last_error()
     assert _sample(L, None) == -1 and b"null" in L.sedd_last_error()
     assert _sample(L, None, M=0) == 0
+    # more rows than one launch has threads for
+    assert _sample(L, ptr, M=1 << 26, Ln=1 << 26, V=65, ld=65, ldu=65) == -1 and b"rows" in L.sedd_last_error()
+    assert _sample(L, ptr, M=1 << 32, Ln=1 << 32) == -1 and b"rows" in L.sedd_last_error()
 
 
 def _fwd(L, p, a_dtype=0, mod_dtype=0, stride=64, p_drop=0.0, w=None, nxt=None, M=4, Ln=2, D=64):
@@ -54,6 +57,7 @@ def test_post_norm_refusals(ptr):
             assert fn(L, ptr, **kw) == rc, (fn, kw)
             assert b"post_norm_residual" in L.sedd_last_error()
         assert fn(L, None) == -1 and fn(L, ptr + 4) == -1  # null, misaligned
+        assert fn(L, ptr, M=1 << 26) == -1 and b"rows" in L.sedd_last_error()
         assert fn(L, None, M=0) == 0
     assert _fwd(L, ptr, w=ptr) == -1 and _bwd(L, ptr, dh=ptr) == -1  # a next norm without its tensors
     assert _bwd(L, ptr, dx1=None) == -1                              # neither gradient
@@ -120,3 +124,10 @@ def test_block_parameters_and_names():
     b = _SEDD(ns(tokens=25, graph=ns(type="absorb"), model=ns(**m, post_norm=True, residual_scale=0.5)))
     assert not any("post_norm" in k for k in a.state_dict()) and a.blocks[0].residual_scale == 1.0
     assert "blocks.1.post_norm2.weight" in b.state_dict() and b.blocks[1].residual_scale == 0.5
+
+
+def test_the_dual_track_model_refuses_what_it_has_not():
+    from protein_lig_sedd_amd.model.transformers_protlig_cross import DualTrackDiffusionTransformer
+    for extra in (dict(post_norm=True), dict(residual_scale=0.9)):
+        with pytest.raises(ValueError, match="dual-track"):
+            DualTrackDiffusionTransformer(dict(model=dict(hidden_size=64, cond_dim=32, n_heads=2, n_blocks=1, dropout=0.0, **extra)), 26, 26)
