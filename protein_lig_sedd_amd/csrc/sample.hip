@@ -405,6 +405,9 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, ui
 // ---- V <= 64: a lane owns a row.  Everything is register arithmetic over the lane's own entries, no cross-lane traffic; the
 // rows of a wave are neighbours in memory, so the loads of a wave cover one stretch of it.  In the middle of a sampler run most
 // rows are not sampled: a block packs those that are to its first lanes, and the waves behind them end.
+// 524288 x 26 bf16: 21 us (86 MB, 4.1 TB/s), with top-p 34 us: there the compare and sum loops over the lane's entries bound it, of
+// which all rows of a wave wait for the one with the most candidates to reject.  A wave per row took 5 times as long: 26 of 64
+// lanes at work, and every sum and maximum six steps across lanes.
 template <typename T, int VP> __device__ __forceinline__ void load_entries(const T* p, int V, float (&x)[VP]) {
     constexpr int E = 16 / sizeof(T);
 #pragma unroll
@@ -550,7 +553,10 @@ __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
     if (on) a.out[row] = ans;
 }
 
-// ---- V > 64: NW waves own a row, its entries in registers (NE per lane, four neighbours at a time).
+// ---- V > 64: NW waves own a row, its entries in registers (NE per lane, four neighbours at a time), so HBM is read once whatever
+// the truncation.  16384 x 2365 bf16: 55 us (233 MB, 4.2 TB/s), top-k 50 59 us, top-p 0.9 82 us, both 66 us; the rest over the
+// 46 us of the bytes is latency: a row's loads, its maximum, each rejection are one after the other, and 128 registers a lane leave
+// four waves on a SIMD to cover them.
 // the best and second best ratio, with the best one's value and index
 struct Best {
     float b1, b2, x;
@@ -632,8 +638,9 @@ template <int NW> struct RowRed {
     }
 };
 // the largest key t with at least k entries at or above it (0: there are not so many), bit by bit down to LOW; exactly k
-// entries above a key end the search early.  Counts are popcounts of compare masks: no arithmetic across lanes.
-template <int LOW, int N, class R> __device__ __forceinline__ uint32_t kth_key(const float (&x)[N], int k, R& red) {
+// entries above a key end the search early.  Counts are popcounts of compare masks: no arithmetic across lanes.  With bits below
+// LOW that are not known t is a bound: at least k entries reach it.
+template <int LOW, int N, class R> __device__ __forceinline__ uint32_t kth_bits(const float (&x)[N], int k, R& red) {
     uint32_t t = 0;
     for (int bit = 31; bit >= LOW; --bit) {
         const uint32_t ct = t | (1u << bit);
@@ -647,7 +654,11 @@ template <int LOW, int N, class R> __device__ __forceinline__ uint32_t kth_key(c
             if (n == k) break;
         }
     }
-    return whole_key<LOW>(t);
+    return t;
+}
+// LOW 0, or 16 where the entries are bf16 numbers: the k-th key itself
+template <int LOW, int N, class R> __device__ __forceinline__ uint32_t kth_key(const float (&x)[N], int k, R& red) {
+    return whole_key<LOW>(kth_bits<LOW>(x, k, red));
 }
 // mass of the k first, where t is their kth_key
 template <int N, class R>
@@ -739,7 +750,8 @@ __device__ __forceinline__ int eliminate(const RowParams& rp, bool cut, const fl
 }
 
 // Where top-k or min-p leaves few entries, they are packed, four to a lane of one wave, and only their noise is read:
-// the k-th largest of the lanes' own maxima is a bound that at least k entries reach (k distinct lanes), usually not many more.
+// the k-th largest of the lanes' own maxima is a bound that at least k entries reach (k distinct lanes), usually not many more;
+// its upper 16 bits do (488 x 32003 fp32, top-k 50: 42 us instead of 44; 14 bits pack too many at top-k 200: 81 us instead of 44).
 #define PACK 256
 template <int NW> struct WideShared {
     static constexpr int ROWS = NW == 1 ? 4 : 1;
@@ -823,7 +835,7 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
                 if (rp.k < V) {
                     if (rp.k <= PACK && rp.k <= NT) {
                         const float lm[1] = {top};
-                        const uint32_t bound = kth_key<LOW>(lm, rp.k, red);
+                        const uint32_t bound = kth_bits<16>(lm, rp.k, red);
                         if (bound) {
                             thr = key_value(bound);
                             n = red.count(reach());
