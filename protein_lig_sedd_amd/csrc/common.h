@@ -86,6 +86,54 @@ __device__ __forceinline__ float dpp_max(float v) {
     v = fmaxf(v, dpp_f<0x143, 0xc>(v, v));
     return lane63(v);
 }
+// the same for 64-bit numbers, their halves moved one by one, and for whole numbers
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_d(double old, double v) {
+    const int lo = __builtin_amdgcn_update_dpp(__double2loint(old), __double2loint(v), CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(__double2hiint(old), __double2hiint(v), CTRL, ROWS, 0xf, false);
+    return __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double lane63(double v) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+__device__ __forceinline__ double dpp_sum(double v) {
+    v += dpp_d<0x111, 0xf>(0.0, v);
+    v += dpp_d<0x112, 0xf>(0.0, v);
+    v += dpp_d<0x114, 0xf>(0.0, v);
+    v += dpp_d<0x118, 0xf>(0.0, v);
+    v += dpp_d<0x142, 0xa>(0.0, v);
+    v += dpp_d<0x143, 0xc>(0.0, v);
+    return lane63(v);
+}
+__device__ __forceinline__ double dpp_max(double v) {
+    v = fmax(v, dpp_d<0x111, 0xf>(v, v));
+    v = fmax(v, dpp_d<0x112, 0xf>(v, v));
+    v = fmax(v, dpp_d<0x114, 0xf>(v, v));
+    v = fmax(v, dpp_d<0x118, 0xf>(v, v));
+    v = fmax(v, dpp_d<0x142, 0xa>(v, v));
+    v = fmax(v, dpp_d<0x143, 0xc>(v, v));
+    return lane63(v);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_i(int old, int v) {
+    return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int dpp_sum(int v) {
+    v += dpp_i<0x111, 0xf>(0, v);
+    v += dpp_i<0x112, 0xf>(0, v);
+    v += dpp_i<0x114, 0xf>(0, v);
+    v += dpp_i<0x118, 0xf>(0, v);
+    v += dpp_i<0x142, 0xa>(0, v);
+    v += dpp_i<0x143, 0xc>(0, v);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int dpp_min(int v) {
+    v = min(v, dpp_i<0x111, 0xf>(v, v));
+    v = min(v, dpp_i<0x112, 0xf>(v, v));
+    v = min(v, dpp_i<0x114, 0xf>(v, v));
+    v = min(v, dpp_i<0x118, 0xf>(v, v));
+    v = min(v, dpp_i<0x142, 0xa>(v, v));
+    v = min(v, dpp_i<0x143, 0xc>(v, v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
 
 // e^sigma - 1 as the reference computes it (graph_lib.py:279-283)
 __device__ __forceinline__ float esigm1f(float s) { return s < 0.5f ? expm1f(s) : expf(s) - 1.0f; }

@@ -71,48 +71,47 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 // u + 1e-10 in 32 bits as the reference's catsample rounds it, kept inside (0, 1] whatever u is
 __device__ __forceinline__ float noise_arg(float u) { return __builtin_amdgcn_fmed3f(u + 1e-10f, 1e-10f, 1.0f); }
 
-// NT threads (a power of two of whole waves) joined over one row in 64 bits
+// NT threads joined over one row in 64 bits; every member is called by all of them.  The sums inside a wave go by DPP moves: by
+// shuffles, through the LDS crossbar at each of six steps, they were most of the time that a near row takes.
 template <int NT> struct Joint {
-    double* sd;  // [NT / 64] each
-    int64_t* si;
+    static constexpr int NW = NT / 64;
+    double* sd;  // [NW] each
+    int* si;
     __device__ __forceinline__ double sum(double v) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-        if constexpr (NT == 64) return v;
+        v = dpp_sum(v);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) sd[threadIdx.x >> 6] = v;
         __syncthreads();
         v = sd[0];
-        for (int w = 1; w < NT / 64; ++w) v += sd[w];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += sd[w];
         return v;
     }
-    __device__ __forceinline__ int64_t isum(int64_t v) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-        if constexpr (NT == 64) return v;
+    __device__ __forceinline__ int isum(int v) {
+        v = dpp_sum(v);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) si[threadIdx.x >> 6] = v;
         __syncthreads();
         v = si[0];
-        for (int w = 1; w < NT / 64; ++w) v += si[w];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v += si[w];
         return v;
     }
     // largest v, lowest index among equals
-    __device__ __forceinline__ void best(double& v, int64_t& i) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const double ov = __shfl_xor(v, o, 64);
-            const int64_t oi = __shfl_xor(i, o, 64);
-            if (ov > v || (ov == v && oi < i)) { v = ov; i = oi; }
-        }
-        if constexpr (NT == 64) return;
+    __device__ __forceinline__ void best(double& v, int& i) {
+        const double top = dpp_max(v);
+        i = dpp_min(v == top ? i : INT32_MAX);
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) { sd[threadIdx.x >> 6] = v; si[threadIdx.x >> 6] = i; }
+        if ((threadIdx.x & 63) == 0) { sd[threadIdx.x >> 6] = top; si[threadIdx.x >> 6] = i; }
         __syncthreads();
         v = sd[0];
         i = si[0];
-        for (int w = 1; w < NT / 64; ++w)
-            if (sd[w] > v || (sd[w] == v && si[w] < i)) { v = sd[w]; i = si[w]; }
+#pragma unroll
+        for (int w = 1; w < NW; ++w) {
+            const double ov = sd[w];
+            const int oi = si[w];
+            if (ov > v || (ov == v && oi < i)) { v = ov; i = oi; }
+        }
     }
 };
 
@@ -183,41 +182,49 @@ template <typename T> __device__ int64_t resolve_lanes64(const SampleArgs& a, in
             S += __hiloint2double(hi, lo);
         }
     }
-    double W = rank < rp.k ? q : 0.0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) W += __shfl_xor(W, o, 64);
+    const double W = dpp_sum(rank < rp.k ? q : 0.0);
     const bool kept = in && (rank == 0 || (rank < rp.k && (!(rp.P < 1.f) || S < (double)rp.P * W) && !(q < (double)rp.m)));
-    double best = kept ? r : -1.0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const double other = __shfl_xor(best, o, 64);
-        best = other > best ? other : best;
-    }
+    const double best = dpp_max(kept ? r : -1.0);
     return __builtin_ctzll(__ballot(kept && r == best));
 }
 // A block with the row's scores, weights and ratios in LDS (V <= STAGED).  kth: what kth_key has found for the row, 0 if it is
-// not known (the search for it in here costs more than all the rest: 20 us of 40 at V = 2365).
+// not known (the search for it in here took more than all the rest: 20 us of 40 at V = 2365).
 #define STAGED 4096
 struct StagedRow {
     double q[STAGED], r[STAGED];
     float x[STAGED];
 };
 template <typename T, int NT>
-__device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b, uint32_t kth, StagedRow& s, double* sd, int64_t* si) {
+__device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b, uint32_t kth, StagedRow& s, double* sd, int* si) {
     Joint<NT> J{sd, si};
     const int lane = threadIdx.x & (NT - 1), V = a.V;
     const T* px = (const T*)a.x + row * a.ld;
     const float* u = a.u + row * a.ldu;
     const RowParams rp = row_params(a, b);
-    const int64_t none = (int64_t)1 << 40;
+    const int none = INT32_MAX;
     __syncthreads();
     double top = -1.0;  // (an order key, so that one reduction serves)
-    int64_t mi = none;
-    for (int j = lane; j < V; j += NT) {
-        const float v = to_f32<T>(px[j]);
-        const uint32_t key = order_key(v);
-        s.x[j] = key ? v : -INFINITY;
-        if (key && (double)key > top) { top = (double)key; mi = j; }
+    int mi = none;
+    {
+        // all loads at once (a thread by itself waits for each), the noise into the place of the ratios
+        constexpr int NE = STAGED / NT;
+        T xe[NE];
+        float ue[NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const int j = i * NT + lane;
+            xe[i] = px[j < V ? j : 0];
+            ue[i] = u[j < V ? j : 0];
+        }
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            const int j = i * NT + lane;
+            const float v = to_f32<T>(xe[i]);
+            const uint32_t key = j < V ? order_key(v) : 0u;
+            s.x[j] = key ? v : -INFINITY;
+            s.r[j] = (double)ue[i];
+            if (key && (double)key > top) { top = (double)key; mi = j; }
+        }
     }
     J.best(top, mi);
     if (mi == none) return row_empty(a);
@@ -227,21 +234,21 @@ __device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b,
         const float v = s.x[j];
         const double q = v == mx ? 1.0 : !(v > -INFINITY) || mx == INFINITY ? 0.0 : exp(((double)v - (double)mx) / (double)rp.T);
         s.q[j] = q;
-        s.r[j] = v > -INFINITY ? q / (1e-10 - log((double)noise_arg(u[j]))) : -1.0;
+        s.r[j] = v > -INFINITY ? q / (1e-10 - log((double)noise_arg((float)s.r[j]))) : -1.0;
     }
     double W = 0.0;
     if (rp.P < 1.f) {
         uint32_t t = kth;  // the k-th largest key, or 0 if there are no k candidates
         for (int bit = 31; !kth && rp.k < V && bit >= 0; --bit) {
             const uint32_t ct = t | (1u << bit);
-            int64_t n = 0;
+            int n = 0;
             for (int j = lane; j < V; j += NT) n += order_key(s.x[j]) >= ct;
             n = J.isum(n);
             if (n >= rp.k) t = ct;
             if (n == rp.k) break;  // (then exactly the k first are at or above t)
         }
         double border = 0.0;
-        int64_t n = 0, any = 0;
+        int n = 0, any = 0;
         for (int j = lane; j < V; j += NT) {
             const uint32_t key = order_key(s.x[j]);
             if (key > t) { W += s.q[j]; ++n; }
@@ -255,10 +262,10 @@ __device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b,
         }
     }
     float cx = -INFINITY;  // what is still possible: ranked before (cx, ci); at first all
-    int64_t ci = -1;
+    int ci = -1;
     for (;;) {
         double best = -1.0;
-        int64_t bi = none;
+        int bi = none;
         for (int j = lane; j < V; j += NT) {
             const float v = s.x[j];
             if (s.r[j] > best && (v > cx || (v == cx && j < ci))) { best = s.r[j]; bi = j; }
@@ -266,7 +273,7 @@ __device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b,
         J.best(best, bi);
         if (bi == none) return mi;  // (cannot be: the first of the order is always kept)
         const float vw = s.x[bi];
-        int64_t rank = 0;
+        int rank = 0;
         double S = 0.0;
         for (int j = lane; j < V; j += NT) {
             const float v = s.x[j];
@@ -284,17 +291,17 @@ __device__ int64_t resolve_staged64(const SampleArgs& a, int64_t row, int64_t b,
 // the entries whose 32-bit ratio comes within twice the tolerance of the largest, usually one or two, and only those are
 // evaluated in 64 bits.
 template <typename T, int NT>
-__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, uint32_t kth, double* sd, int64_t* si) {
+__device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, uint32_t kth, double* sd, int* si) {
     Joint<NT> J{sd, si};
     const int lane = threadIdx.x & (NT - 1), V = a.V;
     const T* px = (const T*)a.x + row * a.ld;
     const float* u = a.u + row * a.ldu;
-    auto score = [&](int64_t j) { return to_f32<T>(px[j]); };
+    auto score = [&](int j) { return to_f32<T>(px[j]); };
     const RowParams rp = row_params(a, b);
-    const int64_t none = (int64_t)1 << 40;
+    const int none = INT32_MAX;
     // the first entry of the order
     double mxd = -1.0;  // (as an order key, so that one reduction serves)
-    int64_t mi = none;
+    int mi = none;
 #pragma unroll 4
     for (int j = lane; j < V; j += NT) {
         const uint32_t key = order_key(score(j));
@@ -311,7 +318,7 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, ui
         if (key == kmax) return 1.0;
         return top_inf ? 0.0 : exp(((double)v - mx) / rT);
     };
-    auto ratio = [&](uint32_t key, float v, int64_t j) { return weight(key, v) / (1e-10 - log((double)noise_arg(u[j]))); };
+    auto ratio = [&](uint32_t key, float v, int j) { return weight(key, v) / (1e-10 - log((double)noise_arg(u[j]))); };
     bool beyond = top_inf;
     const float c = rate_of(rp.T, beyond);
     const bool fast = !beyond;
@@ -322,7 +329,7 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, ui
         if (!kth && rp.k < V) {  // the k-th largest key; 0 if there are no k candidates
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t ct = t | (1u << bit);
-                int64_t n = 0;
+                int n = 0;
 #pragma unroll 4
                 for (int j = lane; j < V; j += NT) n += order_key(score(j)) >= ct;
                 n = J.isum(n);
@@ -331,7 +338,7 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, ui
             }
         }
         double s = 0.0, q = 0.0;
-        int64_t n = 0;
+        int n = 0;
 #pragma unroll 4
         for (int j = lane; j < V; j += NT) {
             const float v = score(j);
@@ -342,20 +349,20 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, ui
         W = J.sum(s);
         if (t) {
             n = J.isum(n);
-            int64_t dummy = 0;
+            int dummy = 0;
             J.best(q, dummy);
             W += (double)(rp.k - n) * q;  // of equal entries at the border the lowest indices are in; they weigh the same
         }
     };
     uint32_t kc = 0xffffffffu;  // what is still possible: ranked before (kc, ic)
-    int64_t ic = none;
+    int ic = none;
     for (;;) {
         double bv = -1.0, least = -1.0;
-        int64_t bi = none;
-        auto possible = [&](uint32_t key, int64_t j) { return key && (key > kc || (key == kc && j < ic) || ic == none); };
-        auto ratio32 = [&](float v, int64_t j) { return (double)(__builtin_amdgcn_exp2f((v - mxf) * c) * inv_noise(u[j])); };
+        int bi = none;
+        auto possible = [&](uint32_t key, int j) { return key && (key > kc || (key == kc && j < ic) || ic == none); };
+        auto ratio32 = [&](float v, int j) { return (double)(__builtin_amdgcn_exp2f((v - mxf) * c) * inv_noise(u[j])); };
         if (fast) {
-            int64_t any = 0;
+            int any = 0;
 #pragma unroll 4
             for (int j = lane; j < V; j += NT) {
                 const float v = score(j);
@@ -377,7 +384,7 @@ __device__ int64_t resolve_row64(const SampleArgs& a, int64_t row, int64_t b, ui
         if (bi == none) return mi;  // (cannot be: the first of the order is always kept)
         const float vw = score(bi);
         const uint32_t kw = order_key(vw);
-        int64_t rank = 0;
+        int rank = 0;
 #pragma unroll 4
         for (int j = lane; j < V; j += NT) {
             const uint32_t key = order_key(score(j));
@@ -939,13 +946,13 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sam
     if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN + (int64_t)t : ans;
 }
 // a block looks through `per` rows (at most 256) and takes those that came near one after the other
-// 512 threads to a row: of one near row the launch takes 7.5 us at V = 2365 and 21 us at V = 9000 (256 threads: 9.5 and 29,
-// 1024: 12 and 21; and where no row is near, 4 us against 4 and 7)
+// 512 threads to a row: one near row takes 6 us more than none at V = 2365 and 11 us more at V = 9000 (256 threads: 8 and 20, 1024:
+// 11 and 13); the launch alone takes 4 us (1024: 5).
 #define NEAR_NT 512
 template <typename T, bool FITS> __global__ void __launch_bounds__(NEAR_NT) sample_near_kernel(SampleArgs a, int per) {
     constexpr int NT = NEAR_NT;
     __shared__ double sd[NT / 64];
-    __shared__ int64_t si[NT / 64];
+    __shared__ int si[NT / 64];
     __shared__ uint64_t s_mask[NT / 64];
     __shared__ uint32_t s_kth[NT];
     const int64_t row0 = (int64_t)blockIdx.x * per, mine = row0 + threadIdx.x;
@@ -974,7 +981,7 @@ template <typename T, bool FITS> __global__ void __launch_bounds__(NEAR_NT) samp
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) sample_row64_kernel(SampleArgs a) {
     __shared__ double sd[NT / 64];
-    __shared__ int64_t si[NT / 64];
+    __shared__ int si[NT / 64];
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const int64_t b = batch_of_row(a, row);
         int64_t got;
@@ -990,7 +997,7 @@ template <typename T, int VP> static void launch_lane(const SampleArgs& a, hipSt
 template <typename T, int NW, int NE> static void launch_wide(const SampleArgs& a, hipStream_t st) {
     constexpr int R = NW == 1 ? 4 : 1;
     hipLaunchKernelGGL((sample_wide_kernel<T, NW, NE>), dim3((unsigned)((a.M + R - 1) / R)), dim3(NW == 1 ? 256 : NW * 64), 0, st, a);
-    int64_t per = (a.M + 511) / 512;  // (a block of the staged form fills half of a CU's LDS: two rounds of blocks at most)
+    int64_t per = (a.M + 255) / 256;  // (256 blocks; 512: a microsecond more where no row is near)
     per = per > 256 ? 256 : per;
     const dim3 grid((unsigned)((a.M + per - 1) / per));
     if (a.V <= STAGED) hipLaunchKernelGGL((sample_near_kernel<T, true>), grid, dim3(NEAR_NT), 0, st, a, (int)per);
@@ -1038,7 +1045,7 @@ extern "C" int sedd_sample_truncated(const void* logits, int dtype, int64_t ld, 
                                      const int64_t* x, int64_t mask_id, const float* move, int64_t* out, int64_t M,
                                      int64_t L, int V, sedd_stream_t stream) {
     SEDD_CHECK_ARG(dtype == SEDD_F32 || dtype == SEDD_BF16, "sample_truncated: unknown dtype %d", dtype);
-    SEDD_CHECK_ARG(M >= 0 && L > 0 && V > 0 && M % L == 0, "sample_truncated: bad sizes M=%ld L=%ld V=%d", (long)M,
+    SEDD_CHECK_ARG(M >= 0 && L > 0 && V > 0 && V <= 1 << 30 && M % L == 0, "sample_truncated: bad sizes M=%ld L=%ld V=%d", (long)M,
                    (long)L, V);
     // (a launch has at most 2^32 - 1 threads: 256 to four rows, or to one above 3000 entries, where memory ends before)
     SEDD_CHECK_ARG(M <= ((int64_t)1 << 26) - 4 || (V <= 64 && M <= ((int64_t)1 << 32) - 256), "sample_truncated: %ld rows of %d entries",

@@ -25,7 +25,7 @@ def _sample(L, p, dtype=0, ld=26, ldu=26, T=1.0, k=0, P=1.0, m=0.0, x=None, move
 
 def test_sample_truncated_refusals(ptr):
     L = _lib()
-    for kw in (dict(dtype=7), dict(M=5), dict(Ln=0), dict(V=0), dict(M=-1), dict(ld=25), dict(ldu=25), dict(T=-1.0),
+    for kw in (dict(dtype=7), dict(M=5), dict(Ln=0), dict(V=0), dict(V=2 ** 30 + 1, ld=2 ** 30 + 1, ldu=2 ** 30 + 1), dict(M=-1), dict(ld=25), dict(ldu=25), dict(T=-1.0),
                dict(T=math.nan), dict(T=math.inf), dict(P=1.5), dict(P=math.nan), dict(m=-0.5), dict(k=-2), dict(move=ptr),
                dict(x=ptr, move=ptr), dict(x=ptr)):  # (the last two: no column for the move numbers; out is x)
         assert _sample(L, ptr, **kw) == -1, kw
