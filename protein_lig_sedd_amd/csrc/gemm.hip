@@ -1749,7 +1749,7 @@ static int gemm_tn_impl(const void* A, int64_t lda, const void* B, int64_t ldb, 
     // A short reduction (the dual-track model at batch 4 reduces over 2048 or 512 tokens) is not split at all: 128-wide
     // tiles, one block per tile walking all of K and adding into C directly.  The same GPU time as split + second pass at
     // these sizes (1024 x 1024 over 2048 tokens: 17 + 10 us -> 27 us) and one launch fewer, which is what counts where
-    // the step is bound by the host's enqueue rate (DESIGN.md section 5).  SEDD_TN_NOSPLIT_KT=0 restores the split.
+    // the step is bound by the host's enqueue rate.  SEDD_TN_NOSPLIT_KT=0 restores the split.
     static const int nosplit_kt = getenv("SEDD_TN_NOSPLIT_KT") ? atoi(getenv("SEDD_TN_NOSPLIT_KT")) : 64;
     const bool nosplit = out_dtype == SEDD_F32 && K / BIG_BK <= nosplit_kt && t128 >= 16;
     // (the 256-wide tile sits at 256 VGPRs: with the column sums' accumulator and selector it spills 71 -> 128-wide then)

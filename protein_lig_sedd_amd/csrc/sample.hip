@@ -147,9 +147,9 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 template <int LOW> __device__ __forceinline__ uint32_t whole_key(uint32_t t) {
     return t && !(t >> 31) ? t | ((1u << LOW) - 1u) : t;
 }
-enum Verdict { KEPT, DROPPED, NEAR };
+enum Decision { KEPT, DROPPED, NEAR };
 // what the 32-bit numbers say about the entry of a given rank, mass before it and weight
-__device__ __forceinline__ Verdict judge(const RowParams& rp, int rank, float S, float W, float q, float best, float second) {
+__device__ __forceinline__ Decision decide(const RowParams& rp, int rank, float S, float W, float q, float best, float second) {
     if (rank != 0) {
         const float margin = rp.P * W - S, tol = MASS_TOL * W;
         if (rank >= rp.k || (rp.P < 1.f && margin < -tol) || q < rp.m * (1.f - RATIO_TOL)) return DROPPED;
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(256) sample_lane_kernel(SampleArgs a) {
             nx = v > n1 ? x[j] : nx;
             n1 = fmaxf(n1, v);
         }
-        const Verdict w = judge(rp, rank, S, W, __builtin_amdgcn_exp2f((xw - mx) * c), b1, b2);
+        const Decision w = decide(rp, rank, S, W, __builtin_amdgcn_exp2f((xw - mx) * c), b1, b2);
         if (open && w != DROPPED) {
             open = false;
             if (w == KEPT) got = iw;
@@ -747,7 +747,7 @@ __device__ __forceinline__ int eliminate(const RowParams& rp, bool cut, const fl
             s += (float)ties * q;
         }
         const int rank = RANK ? above + ties : (v.x == mx ? ties : ties + 1);  // (without RANK only whether it is 0 matters)
-        const Verdict d = judge(rp, rank, s, W, q, v.b1, v.b2);
+        const Decision d = decide(rp, rank, s, W, q, v.b1, v.b2);
         if (d != DROPPED) {
             near = d == NEAR;
             return v.i;

@@ -133,6 +133,24 @@ def test_ties_and_equal_rows(V):
     check(torch.ones(4, V, device=DEV), u1, top_k=2)
 
 
+@pytest.mark.parametrize("V,rows", [(40, 5), (300, 5), (700, 3), (1500, 3), (1500, 520), (2365, 3), (2365, 520), (2900, 520), (3500, 3),
+                                    (6000, 3), (6000, 260), (12000, 3), (12000, 260), (20000, 2), (33000, 2)])
+def test_rows_decided_by_a_tie(V, rows):
+    """the two best ratios equal to the bit (equal scores and noise), alone and where a border runs through them"""
+    from protein_lig_sedd_amd import ops
+    x, u = data((rows, V), torch.float32, V)
+    u[:] = 0.5
+    top, i = x.topk(3, dim=-1)
+    x.scatter_(1, i[:, 1:2], top[:, :1])
+    some = [0, rows - 1]
+    for c in (dict(), dict(top_k=1), dict(top_k=2), dict(top_k=20, top_p=0.9), dict(top_p=0.3), dict(top_k=200, top_p=0.999, min_p=0.01),
+              dict(temperature=3.0, min_p=0.5)):
+        got = ops.sample_truncated(x, u, **c)
+        assert torch.equal(got[some].cpu(), ref(x[some], u[some], c.get("temperature", 1.0), c.get("top_k", 0), c.get("top_p", 1.0),
+                                                c.get("min_p", 0.0))), c
+        assert torch.equal(got, i[:, :2].amin(-1)), c  # the lower index of the two
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [3, 26, 64, 150, 4500])
 def test_masks_and_non_finite(V, dtype):
