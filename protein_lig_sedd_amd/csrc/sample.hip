@@ -187,8 +187,8 @@ template <typename T> __device__ int64_t resolve_lanes64(const SampleArgs& a, in
     const double best = dpp_max(kept ? r : -1.0);
     return __builtin_ctzll(__ballot(kept && r == best));
 }
-// A block with the row's scores, weights and ratios in LDS (V <= STAGED).  kth: what kth_key has found for the row, 0 if it is
-// not known (the search for it in here took more than all the rest: 20 us of 40 at V = 2365).
+// A block with the row's scores, weights and ratios in LDS (V <= STAGED).  kth: what wide_row has found for the row (its t), 0 if it
+// is not known (the search for it in here took more than all the rest: 20 us of 40 at V = 2365).
 #define STAGED 4096
 struct StagedRow {
     double q[STAGED], r[STAGED];
@@ -767,7 +767,8 @@ template <int NW> struct WideShared {
     float red[2][4 * NW];
     int n, ans;
 };
-// the token of a row that is sampled; near: it is not settled; t: the k-th key if it was needed, else 0 (wave 0's is meant)
+// the token of a row that is sampled; near: it is not settled; t: a key that separates the row's k first from the rest (the
+// k-th largest, or one below it that exactly k entries of the row reach) if it was needed, else 0 (wave 0's is meant)
 template <typename T, int NW, int NE>
 __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, int64_t b, WideShared<NW>& sh, bool& near, uint32_t& t) {
     constexpr int NT = NW * 64, LOW = sizeof(T) == 2 ? 16 : 0;
@@ -833,6 +834,7 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
                 // a bound that what is kept reaches
                 float thr = -INFINITY;
                 int n = PACK + 1;
+                uint32_t bound = 0;
                 auto reach = [&]() __attribute__((always_inline)) {
                     int m = 0;
 #pragma unroll
@@ -842,7 +844,7 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
                 if (rp.k < V) {
                     if (rp.k <= PACK && rp.k <= NT) {
                         const float lm[1] = {top};
-                        const uint32_t bound = kth_bits<16>(lm, rp.k, red);
+                        bound = kth_bits<16>(lm, rp.k, red);
                         if (bound) {
                             thr = key_value(bound);
                             n = red.count(reach());
@@ -893,7 +895,10 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
                         }
                         float W = 0.f;
                         if (rp.P < 1.f) {
-                            if (!t) t = kth_key<LOW>(y, rp.k, alone);
+                            // Where exactly k entries are packed, the bound they reach is what separates them.  A search among
+                            // them would end at the first key below them all, which more of the row may reach; of more than k
+                            // it ends above the bound, where the packed entries are all that the row has.
+                            if (!t) t = n == rp.k ? bound : kth_key<LOW>(y, rp.k, alone);
                             W = mass_of_first(y, rp.k, t, mx, c, alone);
                         }
                         got = eliminate<true, 4>(rp, cut, y, ry, [&](int i) { return i == 0 ? jj[0] : i == 1 ? jj[1] : i == 2 ? jj[2] : jj[3]; }, 0,
@@ -929,7 +934,7 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
     }
 }
 
-// A row that came near gets this, and its k-th key in the low half, in place of its token until sample_near_kernel, launched behind, has decided it: kept in this
+// A row that came near gets this, and wide_row's t in the low half, in place of its token until sample_near_kernel, launched behind, has decided it: kept in this
 // kernel, the 64-bit arithmetic would take its registers (115 instead of 60) and half of its waves (131072 x 300: 159 us with it,
 // 79 us and 4 us for the launch behind without), and one wave alone with a row would be the last of the launch by 50 us.
 #define NEAR_TOKEN INT64_MIN
