@@ -95,7 +95,8 @@ int sedd_philox_uniform(uint64_t seed, uint64_t offset, float* u, int64_t M, int
  *   kept = rank < top_k, and sum of q ranked before j < top_p * (sum of q over rank < top_k), and q_j >= min_p; rank 0 always
  *   out  = argmax over kept of q_j / (1e-10 - log(min(u_j + 1e-10, 1)))  (u + 1e-10 rounded to fp32), lowest index of equals
  * as 64-bit arithmetic decides it: rows near a border are decided in 64 bits, so the token depends on neither the kernel
- * variant nor the batch.  T <= 0 (or NaN): the first maximum.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0: off.
+ * variant nor the batch.  T <= 0 (or NaN): the first maximum.  top_k <= 0 or >= V, top_p >= 1 (or NaN), min_p <= 0 (or NaN): off;
+ * top_p <= 0 or min_p > 1 keep rank 0 alone (numbers are held to [0, 1], values in device memory are not looked at).
  * u fp32 [M, V] with row stride ldu, in [0, 1).  temperature / top_p / min_p fp32, top_k int32: one value per batch element
  * (row r belongs to r / L), or NULL: the scalar beside it.  A row with nothing to sample gives -1.
  * x (int64 [M], may be NULL): current tokens — only rows that hold mask_id are sampled, the others keep theirs, and a row with

@@ -857,7 +857,7 @@ __device__ __forceinline__ int64_t wide_row(const SampleArgs& a, int64_t row, in
                         n = red.count(reach());
                     }
                 } else if (!(rp.P < 1.f) && rp.m > 0.f) {
-                    thr = mx + (__builtin_amdgcn_logf(rp.m) - 0.01f) / c;
+                    thr = fminf(mx + (__builtin_amdgcn_logf(rp.m) - 0.01f) / c, mx);  // (a min-p above 1 leaves the maximum)
                     n = red.count(reach());
                 }
                 const bool cut = rp.k < V || rp.P < 1.f || rp.m > 0.f;
