@@ -496,6 +496,10 @@ int sedd_clip_from_sumsq(float* out, float gscale, float max_norm, sedd_stream_t
 #define SEDD_MULTI_WS_DOUBLES 4096
 int sedd_multi_norm_clip(const void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host, int ntensors,
                          float max_norm, double* ws, int64_t ws_doubles, float* out, sedd_stream_t stream);
+/* the same with a max_norm of 64 bits (a HOST number, read before the call returns): the coefficient is rounded once, to fp32.
+ * 0.1 as an fp32 number gives another one for every fifth norm. */
+int sedd_multi_norm_clip_f64(const void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host, int ntensors,
+                             const double* max_norm_host, double* ws, int64_t ws_doubles, float* out, sedd_stream_t stream);
 /* every tensor *= coef[0] in place (fp32 product rounded to the tensor's type); coef is one fp32 on the device, e.g. out + 1 of
  * sedd_multi_norm_clip.  coef == 1 leaves the tensors unread.  round_coef != 0: bf16 tensors are multiplied by the coefficient
  * as bf16 holds it (off by up to 2^-9), the value `grad.mul_(coef)` uses in a loop over the tensors. */

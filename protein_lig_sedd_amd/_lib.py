@@ -85,6 +85,7 @@ SIGNATURES = {
     "sedd_ema_update": "ppflp",
     "sedd_batch_weighted_sum": "ppllppp",
     "sedd_multi_norm_clip": "pppi" + "fplpp",
+    "sedd_multi_norm_clip_f64": "pppi" + "pplpp",
     "sedd_multi_scale": "pppipip",
 }
 

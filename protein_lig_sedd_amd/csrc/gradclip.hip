@@ -167,22 +167,29 @@ static int for_each_table(const void* const* ptrs, const int64_t* numel, const i
     return base;
 }
 
-extern "C" int sedd_multi_norm_clip(const void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host,
-                                    int ntensors, float max_norm, double* ws, int64_t ws_doubles, float* out,
-                                    sedd_stream_t stream) {
+extern "C" int sedd_multi_norm_clip_f64(const void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host,
+                                        int ntensors, const double* max_norm_host, double* ws, int64_t ws_doubles, float* out,
+                                        sedd_stream_t stream) {
     int rc = check_table("multi_norm_clip", ptrs_host, numel_host, dtype_host, ntensors);
     if (rc) return rc;
-    SEDD_CHECK_ARG(max_norm >= 0.f, "multi_norm_clip: max_norm %f", (double)max_norm);
-    SEDD_CHECK_ARG(ws && out, "multi_norm_clip: null pointer");
+    SEDD_CHECK_ARG(ws && out && max_norm_host, "multi_norm_clip: null pointer");
+    const double max_norm = *max_norm_host;
+    SEDD_CHECK_ARG(max_norm >= 0.0, "multi_norm_clip: max_norm %f", max_norm);
     SEDD_CHECK_ARG(ws_doubles >= MULTI_PIECES + (int64_t)ntensors, "multi_norm_clip: workspace of %ld doubles, need %ld",
                    (long)ws_doubles, (long)MULTI_PIECES + ntensors);
     hipStream_t st = (hipStream_t)stream;
     const int n = for_each_table(ptrs_host, numel_host, dtype_host, ntensors, false, [&](const TensorTable& tab, int blocks) {
         hipLaunchKernelGGL(multi_sumsq_kernel, dim3(blocks), dim3(TPB), 0, st, tab, ws);
     });
-    hipLaunchKernelGGL(multi_norm_kernel, dim3(1), dim3(1024), 0, st, ws, n, (double)max_norm, out);
+    hipLaunchKernelGGL(multi_norm_kernel, dim3(1), dim3(1024), 0, st, ws, n, max_norm, out);
     SEDD_LAUNCH_CHECK();
     return SEDD_OK;
+}
+extern "C" int sedd_multi_norm_clip(const void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host,
+                                    int ntensors, float max_norm, double* ws, int64_t ws_doubles, float* out,
+                                    sedd_stream_t stream) {
+    const double limit = max_norm;
+    return sedd_multi_norm_clip_f64(ptrs_host, numel_host, dtype_host, ntensors, &limit, ws, ws_doubles, out, stream);
 }
 
 extern "C" int sedd_multi_scale(void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host, int ntensors,

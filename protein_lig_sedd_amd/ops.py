@@ -1301,8 +1301,9 @@ def _multi_norm(tab, max_norm, device):
     # (allocated per call: two captured graphs, or two streams, never share it)
     ws = torch.empty(4096 + args[3], dtype=torch.float64, device=device)
     out = torch.empty(2, dtype=torch.float32, device=device)
-    check(lib().sedd_multi_norm_clip(*args, max_norm, ws.data_ptr(), ws.numel(), out.data_ptr(), _stream()),
-          "sedd_multi_norm_clip")
+    limit = array.array("d", (max_norm,))
+    check(lib().sedd_multi_norm_clip_f64(*args, limit.buffer_info()[0], ws.data_ptr(), ws.numel(), out.data_ptr(), _stream()),
+          "sedd_multi_norm_clip_f64")
     return out, args
 
 
