@@ -455,6 +455,7 @@ def sample_truncated(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
 def philox_uniform(noise, shape, device):
     """the uniform numbers a PhiloxNoise stands for, as a tensor [..., columns]"""
     u = torch.empty(shape, dtype=torch.float32, device=device)
+    _cuda(u)
     seed = noise.seed - (1 << 64) if noise.seed >= (1 << 63) else noise.seed
     check(lib().sedd_philox_uniform(seed, noise.offset, _p(u), u.numel() // max(shape[-1], 1), shape[-1], _stream()),
           "sedd_philox_uniform")
