@@ -457,8 +457,9 @@ def philox_uniform(noise, shape, device):
     u = torch.empty(shape, dtype=torch.float32, device=device)
     _cuda(u)
     seed = noise.seed - (1 << 64) if noise.seed >= (1 << 63) else noise.seed
-    check(lib().sedd_philox_uniform(seed, noise.offset, _p(u), u.numel() // max(shape[-1], 1), shape[-1], _stream()),
-          "sedd_philox_uniform")
+    with _on_device(u):
+        check(lib().sedd_philox_uniform(seed, noise.offset, _p(u), u.numel() // max(shape[-1], 1), shape[-1], _stream()),
+              "sedd_philox_uniform")
     return u
 
 
