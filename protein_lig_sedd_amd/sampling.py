@@ -153,7 +153,7 @@ def get_sampling_fn(config, graph, noise, batch_dims, eps, device):
                           steps=config.sampling.steps, denoise=config.sampling.noise_removal, eps=eps, device=device, **cut)
 
 
-def _truncation(predictor, graph, temperature, top_k, top_p, min_p):
+def _truncation(predictor, graph, denoise, temperature, top_k, top_p, min_p):
     """the truncation that was asked for, or {} for none; refuses what cannot honour it"""
     cut = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     if not any(torch.is_tensor(v) for v in cut.values()) and (temperature, top_k, top_p, min_p) == (1.0, 0, 1.0, 0.0):
@@ -161,6 +161,9 @@ def _truncation(predictor, graph, temperature, top_k, top_p, min_p):
     if predictor not in ("ancestral", "none"):
         raise ValueError(f"temperature / top_k / top_p / min_p need predictor='ancestral' (or 'none'), got {predictor!r}: the "
                          "Euler and Analytic updates mix the mask state into the distribution that would be truncated")
+    if predictor == "none" and not denoise:
+        raise ValueError("temperature / top_k / top_p / min_p with predictor='none' need the denoising step: without it no token "
+                         "is drawn")
     if not hasattr(graph, "ancestral_step"):
         raise ValueError("temperature / top_k / top_p / min_p need the absorbing graph")
     return cut
@@ -204,14 +207,14 @@ class _GraphedStep:
 
 def get_pc_sampler(graph, noise, batch_dims, predictor, steps, denoise=True, eps=1e-5, device=torch.device('cpu'),
                    proj_fun=lambda x: x, hip_graph=False, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """sampling.py:149-175.  temperature / top_k / top_p / min_p (not in the reference; predictor "ancestral", or "none" for
-    one-shot denoising, absorbing graph): numbers, or device tensors with one value per sequence — the tokens that appear are
+    """sampling.py:149-175.  temperature / top_k / top_p / min_p (not in the reference; predictor "ancestral", or "none" with
+    denoise for one-shot denoising, absorbing graph): numbers, or device tensors with one value per sequence — the tokens that appear are
     drawn from the truncated distribution (ops.sample_truncated).  hip_graph=True (not in the reference): the predictor update is captured once per (model,
     task, conditioning, noise form) as a HIP graph and replayed `steps` times — same kernels, same tokens for the same
     noise; for launch-bound (small) models.  It needs proj_fun and the model's forward to be capturable (device-side
     work only) and takes noise_seq as explicit tensors or None (torch's generator), not as a PhiloxStream (whose offsets
     are host integers)."""
-    truncation = _truncation(predictor, graph, temperature, top_k, top_p, min_p)
+    truncation = _truncation(predictor, graph, denoise, temperature, top_k, top_p, min_p)
     if predictor == "ancestral" and not hasattr(graph, "ancestral_step"):
         raise ValueError("predictor 'ancestral' needs the absorbing graph")
     predictor = get_predictor(predictor)(graph, noise)
