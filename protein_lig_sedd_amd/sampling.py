@@ -123,7 +123,9 @@ class AncestralPredictor(Predictor):
 
     def update_fn(self, score_model, x, t, step_size, task=None, prot_indices=None, lig_indices=None, u=None):
         sigma, nxt = self.noise(t)[0], self.noise(t - step_size)[0]
-        move = (torch.expm1(sigma - nxt) / torch.expm1(sigma)).reshape(-1)
+        # (e^80 is inside fp32's range, e^sigma above 88 is not, and 1 - e^-80 is 1)
+        low, lnxt = sigma.clamp(max=80.0), nxt.clamp(max=80.0)
+        move = (torch.expm1(low - lnxt) / torch.expm1(low)).reshape(-1)
         log_score = model_log_score(score_model, x, sigma, task, prot_indices, lig_indices)
         return self.graph.ancestral_step(log_score, x, move, u=u, **self.truncation)
 
