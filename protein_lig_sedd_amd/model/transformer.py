@@ -163,6 +163,8 @@ class DDiTBlock(nn.Module):
     post_norm2 (LayerNorm with a weight), before their gate, and residual_scale multiplies the residual stream at each of
     the two residuals: x <- residual_scale * x + gate * dropout(post_norm(branch(norm(x))))."""
 
+    residual_scale, param_names = 1.0, Lyr.BLOCK_PARAMS  # (of a block that was pickled before it had its own)
+
     def __init__(self, dim, n_heads, cond_dim, mlp_ratio=4, dropout=0.1, compute_dtype=torch.bfloat16, post_norm=False,
                  residual_scale=1.0):
         super().__init__()
