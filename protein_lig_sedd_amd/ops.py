@@ -834,8 +834,8 @@ def post_norm_residual_bwd(dx1, a, post_w, gate, stats, dgate, dpost_w, keep=Non
         if t is not None and (t.shape != (D,) or t.dtype != torch.float32 or not t.is_contiguous()):
             raise ValueError(f"post_norm_residual_bwd: {n} must be contiguous fp32 [{D}]")
     for t, n in ((dgate, "dgate"), (dshift, "dshift"), (dscale, "dscale")):
-        if t is not None and (t.shape != (B, D) or t.dtype != torch.float32 or t.stride(1) != 1):
-            raise ValueError(f"post_norm_residual_bwd: {n} must be fp32 [{B}, {D}] with contiguous rows")
+        if t is not None and (t.shape != (B, D) or t.dtype != torch.float32 or t.stride(1) != 1 or (B > 1 and t.stride(0) < D)):
+            raise ValueError(f"post_norm_residual_bwd: {n} must be fp32 [{B}, {D}] with contiguous rows of their own")
     gs = dgate.stride(0) if dgate is not None else D
     dms = dshift.stride(0) if dshift is not None else (dscale.stride(0) if dscale is not None else D)
     if dshift is not None and dscale is not None and B > 1 and dscale.stride(0) != dms:
