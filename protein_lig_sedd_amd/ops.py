@@ -773,7 +773,7 @@ def _post_norm_args(name, residual, a, post_w, gate, keep, norm):
     for w in (post_w,) if norm is None else (post_w, norm[0]):
         if w.dtype is not torch.float32 or w.shape != (D,) or not w.is_contiguous():
             raise ValueError(f"{name}: norm weights must be contiguous fp32 [{D}]")
-    ms = gate.stride(0)
+    ms = gate.stride(0) if B > 1 else D
     for t in (gate,) if norm is None else (gate,) + norm[1:]:
         if t.dtype is not gate.dtype or t.shape != (B, D) or t.stride(1) != 1 or (B > 1 and t.stride(0) != ms):
             raise ValueError(f"{name}: gate / shift / scale must be [{B}, {D}] slices of one modulation dtype and row stride")

@@ -46,3 +46,16 @@ def test_one_batch_element_of_any_row_stride():
     dgate = torch.zeros(D, device=DEV).as_strided((1, D), (0, 1))
     ops.post_norm_residual_bwd(s["dx1"], s["a"], s["post_w"], s["gate"], stats, dgate, None)
     assert torch.equal(dgate, want)
+
+
+def test_modulation_of_one_batch_element_and_any_row_stride():
+    """one row has no next one, so its stride means nothing"""
+    L, D = 5, 64
+    s = make(1, L, D, torch.float32)
+    odd = {n: torch.cat([s[n], torch.zeros(1, 1, device=DEV)], 1)[:, :D] for n in ("gate", "shift", "scale")}
+    assert all(t.stride(0) == D + 1 for t in odd.values())
+    x1, h, stats = run_fwd(s, 1.0, True)
+    y1, g, other = run_fwd({**s, **odd}, 1.0, True)
+    assert torch.equal(x1, y1) and torch.equal(h, g)
+    want, got = run_bwd(s, 1.0, True, x1, stats), run_bwd({**s, **odd}, 1.0, True, y1, other)
+    assert all(torch.equal(want[k], got[k]) for k in want)
