@@ -502,7 +502,7 @@ int sedd_multi_norm_clip_f64(const void* const* ptrs_host, const int64_t* numel_
                              const double* max_norm_host, double* ws, int64_t ws_doubles, float* out, sedd_stream_t stream);
 /* every tensor *= coef[0] in place (fp32 product rounded to the tensor's type); coef is one fp32 on the device, e.g. out + 1 of
  * sedd_multi_norm_clip.  coef == 1 leaves the tensors unread.  round_coef != 0: bf16 tensors are multiplied by the coefficient
- * as bf16 holds it (off by up to 2^-9), the value `grad.mul_(coef)` uses in a loop over the tensors. */
+ * as bf16 holds it (off by up to 2^-8), the value `grad.mul_(coef)` uses in a loop over the tensors. */
 int sedd_multi_scale(void* const* ptrs_host, const int64_t* numel_host, const int32_t* dtype_host, int ntensors,
                      const float* coef, int round_coef, sedd_stream_t stream);
 

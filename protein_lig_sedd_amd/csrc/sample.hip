@@ -124,7 +124,8 @@ template <int NT> struct Joint {
 //   S, W: sum q |d2| <= W log2 V, so a sum is off by (log2 V * 2.8 + 2) 2^-24 W and by its n adds one after the other, n 2^-24 W:
 //     V <= 64 in one lane 5.0e-6 W; 64 a lane and 10 across, V = 32768: 7.1e-6 W.  S against P W: 1.42e-5 W at most: MASS_TOL.
 // Both tolerances are 1.53e-5.  A comparison nearer than that, and every row whose maximum or temperature leaves the range of
-// these bounds, is "near": about one row in 30000 with top-p.
+// these bounds, is "near".  Counted over normal scores: with top-p one row in 22000 to 38000 at V = 26, in 7000 to 49000 from V = 300
+// on, at top-p 0.3 (the answer changes more often there) in 5000 to 24000; without top-p one in 49000 or fewer.
 #define RATIO_TOL 0x1p-16f
 #define MASS_TOL 0x1p-16f
 #define LOG2E 1.44269504f
@@ -951,8 +952,9 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 64, NE <= 40 ? 4 : 2) sam
     if (NW == 1 ? (threadIdx.x & 63) == 0 : threadIdx.x == 0) a.out[row] = near ? NEAR_TOKEN + (int64_t)t : ans;
 }
 // a block looks through `per` rows (at most 256) and takes those that came near one after the other
-// 512 threads to a row: one near row takes 6 us more than none at V = 2365 and 11 us more at V = 9000 (256 threads: 8 and 20, 1024:
-// 11 and 13); the launch alone takes 4 us (1024: 5).
+// 512 threads to a row: where a single row was sampled and its scores lie in the L2, a near row takes 6 us more than none at V = 2365
+// and 11 us more at V = 9000 (256 threads: 8 and 20, 1024: 11 and 13).  Behind 16384 x 2365 bf16 the launch takes 4 to 5 us if no row
+// is near, 12 to 16 with one (read from HBM) and 15 to 21 with three.
 #define NEAR_NT 512
 template <typename T, bool FITS> __global__ void __launch_bounds__(NEAR_NT) sample_near_kernel(SampleArgs a, int per) {
     constexpr int NT = NEAR_NT;
@@ -1028,6 +1030,11 @@ template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t
     //   V =  3900:    64 rows 46 / 20 | 58 / 26;  512 rows 69 / 27 | 86 / 31;  8192 rows 188 / 105 | 248 / 196
     //   V = 12000:    64 rows 61 / 38 | 76 / 45;  256 rows 60 / 38 | 95 / 52;  2048 rows 218 / 174 | 274 / 405
     // (V = 600: no difference up to 512 rows.)
+    // 40 entries a lane are the most for four waves on a SIMD (128 registers), 48 the most for three (167; 52 a lane leave two:
+    // 392 us instead of 284 at V = 2900), and as far as that goes one wave is no worse where rows are many.  8192 rows, top-p 0.9 | top-p 0.3 |
+    // top-k 500 and top-p 0.3 | top-k 50 and top-p 0.9, one wave / four waves:
+    //   V = 1500:  39 / 41 |  79 / 77  |  79 / 102 | 31 / 63      V = 2365:  49 / 64 |  92 / 116 | 102 / 157 | 37 / 76
+    //   V = 2560:  47 / 63 |  80 / 98  | 118 / 175 | 36 / 76      V = 2999:  77 / 80 | 124 / 124 | 137 / 158 | 66 / 93
     else if (a.V > 1024 && a.V <= 2048 && a.M <= 512) launch_wide<T, 4, 8>(a, st);
     else if (a.V > 2048 && a.V <= 4096 && (a.M <= 512 || a.V > 3000)) launch_wide<T, 4, 16>(a, st);
     else if (a.V > 4096 && a.V <= 8192 && a.M <= 256) launch_wide<T, 16, 8>(a, st);
@@ -1041,6 +1048,9 @@ template <typename T> static void launch_sample(const SampleArgs& a, hipStream_t
     else if (a.V <= 8192) launch_wide<T, 4, 32>(a, st);
     else if (a.V <= 16384) launch_wide<T, 4, 64>(a, st);
     else if (a.V <= 32768) launch_wide<T, 16, 32>(a, st);
+    // A longer row does not fit a block's registers and is decided in 64 bits throughout, read again in every pass.  us, fp32, all
+    // kept | top-p 0.9 | top-k 50 and top-p 0.9:  1 x 33001  37 | 62 | 156;  488 x 33001  122 | 325 | 680 (488 x 32003 above: 37 | 51 | 44);
+    // 256 x 131071  237 | 726 | 1945
     else hipLaunchKernelGGL((sample_row64_kernel<T, 1024>), dim3(sedd_grid_for(a.M, 1, 512)), dim3(1024), 0, st, a);
 }
 

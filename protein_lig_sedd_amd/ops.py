@@ -1323,7 +1323,7 @@ def clip_grad_norm_(grads, max_norm, error_if_nonfinite=False, round_coef=False)
     """Scale a list of fp32 / bf16 gradient tensors in place by min(1, max_norm / (norm + 1e-6)), norm = their joint 2-norm
     -> the norm before clipping, a 0-dim fp32 tensor on the device (not read on the host, except to raise under
     error_if_nonfinite, before anything is scaled).  round_coef=True multiplies bf16 tensors by the coefficient as bf16 holds it
-    (off by up to 2^-9): bit parity with a loop of `grad.mul_(coef)`.  torch.nn.utils.clip_grad_norm_ on the gradients themselves (losses.py:65-66)."""
+    (off by up to 2^-8): bit parity with a loop of `grad.mul_(coef)`.  torch.nn.utils.clip_grad_norm_ on the gradients themselves (losses.py:65-66)."""
     grads = [grads] if torch.is_tensor(grads) else list(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0:
