@@ -343,7 +343,7 @@ __device__ __forceinline__ void stage_put4(unsigned char* reg, int row_l, int co
     store_row4<TO>(reinterpret_cast<TO*>(reg + row_l * StageCfg<TO>::PITCH) + col_l, v);
 }
 // flush one pass: rows [row_g, row_g + RPP) x columns [col_g, col_g + 64) of C; accumulate adds the old C (fp32/bf16)
-// (Round 2 tried to take the per-chunk 64-bit row * ldc multiplies and bound compares out of the pass loops — a per-tile
+// (Tried: taking the per-chunk 64-bit row * ldc multiplies and bound compares out of the pass loops — a per-tile
 // lane context with wave-uniform pass offsets, then with running pointers: the first form had the compiler hoist a
 // (pass, group) table of 64-bit offsets into SGPRs and spill 136-152 of them to VGPR lanes, the second spilled 14-82
 // VGPRs in the 256-wide kernels, which sit at the 256-register limit; both measured slower — fc1 epilogue 10.4 -> 12.6 us
@@ -1312,7 +1312,7 @@ static int choose_csplit(int64_t tm, int64_t tn, int64_t tiles, int64_t M, int64
 static void big_splitk(int64_t tiles, int64_t K, int* splitk, int64_t* kper) {
     const int64_t nkt = K / BIG_BK;
     static const int min_kt = getenv("SEDD_SPLITK_MIN_KT") ? atoi(getenv("SEDD_SPLITK_MIN_KT")) : 8;  // K tiles per slice at least
-    // (A/B knob; 16 -> 8 in round 3: the dual-track model's weight gradients reduce over 2048 or 512 tokens only, cfg 3
+    // (A/B knob; 8 instead of 16: the dual-track model's weight gradients reduce over 2048 or 512 tokens only, cfg 3
     // bf16 batch 4 38.1 -> 36.7 ms; 4 is slower again — slab traffic; cfg 2 / 4 reduce over >= 16 k tokens: not binding)
     int64_t sk = tiles > 0 ? cu_budget() / tiles : 1;
     if (sk > nkt / min_kt) sk = nkt / min_kt;

@@ -514,8 +514,8 @@ extern "C" int sedd_gumbel_argmax(const void* p, int dtype, const float* u, int6
 // Euler (sampling.py:61-80): p = onehot(x) + dt*dsigma * reverse_rate(x, exp(logscore))   (graph_lib.py:79-96)
 // Analytic (sampling.py:90-99) / Denoiser (:107-132): p = staggered_score(exp(logscore), ds) *
 // transp_transition(x, ds) (graph_lib.py:264-269, :226-234 | :162-165, :147-154), Denoiser drops the mask column.
-// then catsample.py:12-13.  Unmasked rows of the absorbing graph are fixed points (SURVEY section 4
-// KAT-unmasked-fixed-point): p is a one-hot at x, so neither the row's scores nor its noise are read.
+// then catsample.py:12-13.  Unmasked rows of the absorbing graph are fixed points
+// (p is a one-hot at x), so neither the row's scores nor its noise are read.
 template <typename T, int G>
 __global__ void __launch_bounds__(TPB) predictor_step_kernel(int graph, int step, const T* __restrict__ ls,
                                                              const int64_t* __restrict__ x,
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(TPB) predictor_step_kernel(int graph, int step
     }
 }
 
-// What bounds this kernel (round-2 measurements at the cfg-5 shard, 512 x 1024 rows, V = 26, bf16; 90 MB algorithmic):
+// What bounds this kernel (measured at 512 x 1024 rows, V = 26, bf16; 90 MB algorithmic):
 // LDS-DMA alone moves the tiles in 13.5 us, but SQ_INSTS_VALU is 11.4 M wave-instructions per launch — ~2000 per
 // surviving row (OCML expf 13, compensated log 9, IEEE division 11, selects / compares / moves ~25 per vocabulary entry)
 // — and a SIMD issues one VALU instruction per 4 cycles: a ~19 us VALU floor, above the HBM floor.  Persistent variants

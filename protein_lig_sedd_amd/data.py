@@ -1,4 +1,4 @@
-"""Host side of the data path that feeds the hot path (SURVEY 8f4) — the parts that need no downloads:
+"""Host side of the data path that feeds the hot path — the parts that need no downloads:
 
   * fixed-pad batches: what the reference's tokenizer calls produce (`padding='max_length', max_length=512 | 128,
     truncation=True`, data/tokenize.py:14,25) from already-tokenised id lists;

@@ -2,7 +2,7 @@
 (protlig_dd/model/transformers_protlig_cross.py:237-320 `DDiTBlock`, :107-140 `CrossAttentionLayer`) on the HIP
 kernels.  Reproduces the reference AS WRITTEN:
 
-  * quirk Q1: the "self-attention" nn.MultiheadAttention is built with batch_first=True but is fed
+  * the "self-attention" nn.MultiheadAttention is built with batch_first=True but is fed
     [L, B, D] tensors (:301-305), so it attends over the BATCH axis for every sequence position.  Here that is the same
     strided attention kernel called with (batch stride, sequence stride) swapped — no transposes are materialised.
     `seq_axis_attention=True` selects the intended sequence-axis attention instead.

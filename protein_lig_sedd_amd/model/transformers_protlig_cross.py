@@ -189,7 +189,7 @@ class ProteinLigandDiffusionModel(nn.Module):
                                                          seq_axis_attention=seq_axis_attention)
         self._ctx_step, self._ctx_cache, self.context_cache_hits = None, {}, 0
 
-    # ---- per-step context cache for the *_given_* sampling modes -----------------------------------------
+    # ---- per-step context cache for the *_given_* sampling modes ---------------------------------------------------------
     def sampling_step(self, step):
         """Called by sampling.get_pc_sampler's loop: `step` = index of the sampler update about to run (None = sampling
         over).  The conditioning context depends on sigma(t_step), so it is valid for ONE step only: every model call

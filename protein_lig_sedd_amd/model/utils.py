@@ -14,7 +14,7 @@ def _accepts_task(model):
 
 def get_model_fn(model, train=False):
     """model/utils.py:5-37.  The reference forwards prot_seq / lig_seq / task keyword arguments that its own
-    SEDD.forward does not accept (SURVEY 3.1); they are passed only to models whose forward takes them."""
+    SEDD.forward does not accept; they are passed only to models whose forward takes them."""
     takes_task = _accepts_task(model)
 
     def model_fn(x, sigma, prot_seq=None, lig_seq=None, task="ligand_given_protein"):

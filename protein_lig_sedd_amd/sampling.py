@@ -4,11 +4,11 @@ get_pc_sampler / get_sampling_fn — with each update step running as ONE fused 
 
 Differences from the reference, all additive:
   * `u=` (optional) on every update_fn and `noise_seq=` on pc_sampler supply the uniform noise, so identical noise
-    tensors give bit-identical indices (north_star); default None draws torch.rand on the device.
+    tensors give bit-identical indices; default None draws torch.rand on the device.
   * the score model may be either the dual-track cross model (keyword call with `mode=task`, sampling.py:64-76) or a
     plain SEDD (`model(x, sigma)`); the reference's loop only supports the former.
   * AnalyticPredictor accepts both its upstream positional signature `update_fn(score_fn, x, t, step_size)` and the
-    keyword signature pc_sampler uses, so `predictor="analytic"` works through get_pc_sampler (SURVEY quirk Q5: in
+    keyword signature pc_sampler uses, so `predictor="analytic"` works through get_pc_sampler (in
     the reference that call raises TypeError).
 """
 import abc

@@ -92,7 +92,7 @@ def init_distributed():
     if torch.cuda.is_available():
         if backend != "nccl":
             # gloo stages device tensors through the host from its own threads; on this stack every such all-reduce of
-            # a buffer that the launch stream is still writing hung (round-1 rehearsals, also with plain torch ops and
+            # a buffer that the launch stream is still writing hung (also with plain torch ops and
             # none of this package's kernels).  The collectives of this path are RCCL's; gloo is for CPU tensors.
             raise RuntimeError(f"init_distributed: backend {backend!r} cannot carry GPU tensors here — use 'nccl' "
                                "(RCCL); gloo is supported for CPU tensors only")
@@ -198,7 +198,7 @@ class SEDDTrainer:
         # wgrad_stream: weight- and bias-gradient launches of backward go to a second stream (ops.SideStream) and run
         # beside the data-gradient chain — for steps whose kernels each fill a fraction of the chip.  True / False, or None
         # (default) = where it was measured to pay on every box: fp32 compute and steps of at most `_side_max` tokens
-        # (8192).  BASELINE cfg 1 (1024 tokens), same-box A/B x3: fp32 7.94 -> 7.19 ms; bf16 5.2 -> 5.55 ms — that step is
+        # (8192).  The 1024-token step of the D 768 x 8 model, same-box A/B x3: fp32 7.94 -> 7.19 ms; bf16 5.2 -> 5.55 ms — that step is
         # bound by the host's enqueue rate, which the forks add to (on a faster host the same A/B read 5.3 -> 4.9 ms), so
         # bf16 stays opt-in here; at cfg 2's 32768 tokens every GEMM fills the chip and it buys 0.5 %.
         if os.environ.get("SEDD_WGRAD_STREAM") in ("0", "1"):  # (A/B override)
@@ -636,7 +636,7 @@ def shard_batch(batch, rank, world):
 
 def sharded_sampling(sampler, model, rank, world, gather=True, **kw):
     """Batch-sharded sampling: every rank samples its own shard with no communication during the steps; one final
-    all_gather of the int64 indices (SURVEY 8e)."""
+    all_gather of the int64 indices."""
     x = sampler(model, **kw)
     if world == 1 or not gather:
         return x
